@@ -21,10 +21,15 @@ RL_ERR_BAD_VARIANT = -7
 RL_ERR_TENSOR_MAP = -8
 RL_ERR_DEVICE_TIMEOUT = -9
 RL_ERR_STATIC_SCRATCH = -10
+RL_ERR_BAD_INDEX = -11
+RL_ERR_OVERLAP = -12
+RL_ERR_BAD_ACTIVATION = -13
 RL_ERR_CUDA = -1000
 
 RL_W_BF16 = 0
 RL_W_E4M3 = 1
+
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 VARIANTS = {
     "auto": 0,
@@ -63,6 +68,12 @@ SYMBOLS = [
     ("rl_rmsnorm_swiglu_bf16", _i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _f, _vp, _sz, _vp]),
     ("rl_gemm_bf16", _i, [_vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _vp, _sz, _vp]),
     ("rl_lora_linear_bf16", _i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    ("rl_linear_workspace_bytes", _sz, [_i, _i]),
+    ("rl_linear_bf16", _i, [_vp] * 5 + [_i] * 3 + [_i64] * 4 + [_i, _vp, _sz, _i, _vp]),
+    ("rl_qk_norm_rope_bf16", _i, [_vp] * 6 + [_i, _vp, _vp] + [_i] * 6 + [_i64] * 9 + [_f, _i, _vp]),
+    ("rl_kv_cache_write_e4m3", _i, [_vp] * 3 + [_i] + [_vp] * 4 + [_i] * 5 + [_i64] * 10 + [_vp]),
+    ("rl_kv_cache_read_e4m3", _i, [_vp] * 8 + [_i] * 4 + [_i64] + [_i] * 4 + [_i64] * 10 + [_vp]),
+    ("rl_take_index_status", _i, [ctypes.POINTER(ctypes.c_int)]),
     ("rl_selftest_wait_timeout", _i, [_vp, _sz, ctypes.c_ulonglong, _vp]),
     ("rl_read_status", _i, [_vp, ctypes.POINTER(ctypes.c_int)]),
 ]
@@ -98,6 +109,6 @@ def check(code: int, what: str) -> None:
         return
     msg = f"{what}: {error_string(code)} (code {code})"
     if code in (RL_ERR_NULL_POINTER, RL_ERR_BAD_SHAPE, RL_ERR_ALIGNMENT, RL_ERR_BAD_DTYPE, RL_ERR_BAD_VARIANT,
-                RL_ERR_STATIC_SCRATCH):
+                RL_ERR_STATIC_SCRATCH, RL_ERR_OVERLAP, RL_ERR_BAD_ACTIVATION):
         raise ValueError(msg)
     raise RuntimeError(msg)

@@ -4,9 +4,13 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 #include <mutex>
+#include <utility>
 
 #include "rl_decode.cuh"
+#include "rl_kv_cache.cuh"
+#include "rl_qk_rope.cuh"
 #include "rl_rowquant.cuh"
 #include "rl_prefill.cuh"
 #include "rl_prefill_pair.cuh"
@@ -206,6 +210,8 @@ using PairSwigluWide = PairCfg<512, 2, 4, 1, 0, A_SS_DIRECT, true, true>;  // 25
 using PairSwiglu = PairCfg<256, 1, 6, 6, 2, A_TS_FOLD, true, true>;
 using PairSwigluDirect = PairCfg<256, 2, 6, 1, 0, A_SS_DIRECT, true, true>;  // no gamma, or gamma folded by the pre-pass
 using PairFp8 = PairCfg<256, 2, 6, 1, 0, A_SS_DIRECT, true, false, true>;
+using PairLinear = PairCfg<256, 2, 6, 1, 0, A_SS_DIRECT, true, false, false, true>;      // bias, activation, residual
+using PairLinearWide = PairCfg<512, 2, 4, 1, 0, A_SS_DIRECT, true, false, false, true>;
 
 template <class Cfg>
 int launch_prefill(const void* x, const __nv_bfloat16* gamma, const void* W, void* y, int M, int N, int K,
@@ -340,6 +346,10 @@ struct PairArgs {
   int64_t ldx2 = 0, ldw2 = 0;
   const float* row_scale = nullptr;    // FP8: per-token scale (already computed on `st`)
   const float* w_scale = nullptr;      // FP8: per-channel weight scales
+  const __nv_bfloat16* bias = nullptr;      // linear epilogue
+  const __nv_bfloat16* residual = nullptr;
+  int64_t ld_res = 0;
+  int act = 0;
 };
 
 template <class Cfg>
@@ -379,6 +389,13 @@ int launch_prefill_pair(const PairArgs& a) {
   p.status = a.status;
   p.extra_kb = (a.x2 != nullptr) ? 1 : 0;
   p.w_scale = a.w_scale;
+  if (Cfg::EPI) {
+    p.bias = a.bias;
+    p.residual = a.residual;
+    p.ld_res = a.ld_res;
+    p.res_vec = (a.ld_res & 7) == 0 && aligned16(a.residual);
+    p.act = a.act;
+  }
   if (Cfg::FP8) {
     if (a.row_scale == nullptr || a.w_scale == nullptr) return RL_ERR_NULL_POINTER;
     p.row_rstd = a.row_scale;
@@ -461,12 +478,14 @@ using DecodeCfg16 = DecodeCfg<16, RL_DEC16_STAGES, RL_DEC16_TW, RL_DEC16_MINB>;
 template <class Cfg>
 int launch_decode(const void* x, const __nv_bfloat16* gamma, const void* W, void* y, int M, int N, int K,
                   int64_t ldx, int64_t ldw, int64_t ldy, float eps, uint8_t* ws, const WsLayout& wl, int sms,
-                  cudaStream_t st, const float* row_scale = nullptr, const float* w_scale = nullptr) {
+                  cudaStream_t st, const float* row_scale = nullptr, const float* w_scale = nullptr,
+                  const PairArgs* epilogue = nullptr) {
   CUtensorMap tw, tx;
   int rc;
   const CUtensorMapDataType dt = Cfg::FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int eb = Cfg::FP8 ? 1 : 2;
   if (Cfg::FP8 && (!row_scale || !w_scale)) return RL_ERR_NULL_POINTER;
+  if (Cfg::LINEAR && !epilogue) return RL_ERR_BAD_VARIANT;
   if ((rc = make_map(&tw, dt, eb, W, K, N, ldw, Cfg::KBW, 128))) return rc;
   if ((rc = make_map(&tx, dt, eb, x, K, M, ldx, Cfg::KBW, Cfg::MPAD))) return rc;
   DecodeParams p{};
@@ -474,6 +493,12 @@ int launch_decode(const void* x, const __nv_bfloat16* gamma, const void* W, void
   p.gamma = gamma;
   p.row_scale = row_scale;
   p.w_scale = w_scale;
+  if (Cfg::LINEAR) {
+    p.bias = epilogue->bias;
+    p.residual = epilogue->residual;
+    p.ld_res = epilogue->ld_res;
+    p.act = epilogue->act;
+  }
   p.y = reinterpret_cast<__nv_bfloat16*>(y);
   p.ldy = ldy;
   p.n_tiles = (N + 127) / 128;
@@ -626,6 +651,128 @@ int auto_variant(int M, int N, int K, bool has_gamma, bool has_workspace, bool w
   return RL_VARIANT_PREFILL_PAIR_WIDE;
 }
 
+// ---- which memory a strided tensor covers: outputs must not share any with inputs or with one another
+struct View {
+  uintptr_t at = 0;
+  int nd = 0;
+  int64_t n[4], s[4];  // sizes and strides in bytes, largest stride first; the last dimension is the contiguous row
+  bool empty = false;
+  View(const void* p, int elem, std::initializer_list<std::pair<int64_t, int64_t>> dims) : at(reinterpret_cast<uintptr_t>(p)) {
+    for (const auto& d : dims) {  // (size, stride in elements); the strides need not come in order
+      if (d.first <= 0) empty = true;
+      if (d.first <= 1) continue;
+      int i = nd++;
+      for (; i > 0 && s[i - 1] < d.second * elem; --i) { n[i] = n[i - 1]; s[i] = s[i - 1]; }
+      n[i] = d.first;
+      s[i] = d.second * elem;
+    }
+    bytes = elem;
+  }
+  int64_t bytes;
+  int64_t span(int from = 0) const {  // bytes from the first to the end of the last element, dimensions from..
+    int64_t e = bytes;
+    for (int i = from; i < nd; ++i) e += (n[i] - 1) * s[i];
+    return e;
+  }
+  bool self_overlaps() const {
+    for (int i = 0; i < nd; ++i)
+      if (s[i] < span(i + 1)) return true;
+    return false;
+  }
+  bool same(const View& o) const {
+    if (at != o.at || nd != o.nd || bytes != o.bytes) return false;
+    for (int i = 0; i < nd; ++i)
+      if (n[i] != o.n[i] || s[i] != o.s[i]) return false;
+    return true;
+  }
+};
+
+// True only if no byte is shared: the ranges are apart, or the two are interleaved windows of one larger array (equal
+// outer strides, windows apart within a period) - q, k and v inside the rows of one projection, say.
+bool disjoint(const View& a, const View& b, int i = 0, int j = 0, int64_t shift = 0, bool nested = false) {
+  if (a.empty || b.empty) return true;
+  const int64_t d = nested ? shift : (int64_t)(b.at - a.at);  // b's start relative to a's
+  const int64_t wa = a.span(i), wb = b.span(j);
+  if (d >= wa || -d >= wb) return true;
+  if (i >= a.nd || j >= b.nd || a.s[i] != b.s[j]) return false;
+  const int64_t S = a.s[i], ia = a.span(i + 1), ib = b.span(j + 1);
+  if (ia > S || ib > S) return false;
+  const int64_t r = ((d % S) + S) % S;
+  if (r >= ia && r + ib <= S) return true;
+  if (r + ib <= S) return disjoint(a, b, i + 1, j + 1, r, true);            // b's window lies in the same period as a's
+  if (ia <= r) return disjoint(a, b, i + 1, j + 1, r - S, true);            // ... or reaches into a's next one
+  return false;
+}
+
+// A row kernel's launch: `rows` rows of 8-channel chunks per token, one warp per (token, part).
+// Rows of D channels take G lanes, 32 / G rows per step.
+inline int lanes_per_row(int D) {
+  int g = 2;
+  while (g * 8 < D) g *= 2;
+  return g;
+}
+template <class Params, class Kernel>
+int launch_rows(Kernel kernel, Params& p, int tokens, int rows, int G, cudaStream_t st) {
+  const int R = 32 / G;
+  const int groups = (rows + R - 1) / R;
+  p.steps = 1;
+  p.parts = (groups + p.steps - 1) / p.steps;
+  const long long blocks = ((long long)tokens * p.parts + 3) / 4;
+  if (blocks > 0x7fffffffLL) return RL_ERR_BAD_SHAPE;
+  // a programmatic dependent: the kernel touches no global memory before griddepcontrol.wait
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)blocks);
+  lc.blockDim = dim3(128);
+  lc.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = at;
+  lc.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&lc, kernel, p);
+  return e == cudaSuccess ? RL_OK : cuda_err(e);
+}
+#define RL_BY_LANES(G, CALL)        \
+  switch (G) {                      \
+    case 2: return CALL(2);         \
+    case 4: return CALL(4);         \
+    case 8: return CALL(8);         \
+    case 16: return CALL(16);       \
+    default: return CALL(32);       \
+  }
+
+inline bool mult8(std::initializer_list<int64_t> v) {
+  for (int64_t x : v)
+    if (x & 7) return false;
+  return true;
+}
+inline bool nonneg(std::initializer_list<int64_t> v) {
+  for (int64_t x : v)
+    if (x < 0) return false;
+  return true;
+}
+
+// what the two cache entry points check about the cache itself
+int check_cache(const KvCache& c) {
+  if (!c.k_codes || !c.v_codes || !c.k_scale || !c.v_scale) return RL_ERR_NULL_POINTER;
+  if (c.num_pages < 0 || c.page_size <= 0 || c.H <= 0 || c.D <= 0 || c.D > 256 ||
+      !nonneg({c.c_page, c.c_off, c.c_head, c.s_page, c.s_off, c.s_head}))
+    return RL_ERR_BAD_SHAPE;
+  const uintptr_t codes = reinterpret_cast<uintptr_t>(c.k_codes) | reinterpret_cast<uintptr_t>(c.v_codes);
+  const uintptr_t scales = reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale);
+  if ((codes & 7) || (scales & 3) || !mult8({c.D, c.c_page, c.c_off, c.c_head})) return RL_ERR_ALIGNMENT;
+  return RL_OK;
+}
+View code_view(const KvCache& c, const void* p) {
+  return View(p, 1, {{c.num_pages, c.c_page}, {c.page_size, c.c_off}, {c.H, c.c_head}, {c.D, 1}});
+}
+View scale_view(const KvCache& c, const void* p) {
+  return View(p, 4, {{c.num_pages, c.s_page}, {c.page_size, c.s_off}, {c.H, c.s_head}});
+}
+View head_view(const void* p, int T, int H, int D, int64_t st, int64_t sh) {
+  return View(p, 2, {{T, st}, {H, sh}, {D, 1}});
+}
+
 }  // namespace
 
 extern "C" {
@@ -647,6 +794,9 @@ const char* rl_error_string(int code) {
     case RL_ERR_DEVICE_TIMEOUT: return "a bounded wait inside a kernel ran out of time";
     case RL_ERR_STATIC_SCRATCH:
       return "shape exceeds the built-in scratch of the allocation-free entry point (M <= 16 tokens)";
+    case RL_ERR_BAD_INDEX: return "a position, slot or page lay outside its table";
+    case RL_ERR_OVERLAP: return "an output shares memory with an input, another output or itself";
+    case RL_ERR_BAD_ACTIVATION: return "unknown activation";
     default: break;
   }
   if (code <= RL_ERR_CUDA) return cudaGetErrorString((cudaError_t)(RL_ERR_CUDA - code));
@@ -933,6 +1083,186 @@ int rl_lora_linear_bf16(const void* a, const void* b, const void* xa, const void
   pa.no_norm = true;
   pa.x2 = xa; pa.w2 = lb; pa.L = L; pa.ldx2 = ldxa; pa.ldw2 = ldlb;
   return launch_prefill_pair<PairDirect>(pa);
+}
+
+size_t rl_linear_workspace_bytes(int M, int N) {
+  if (M <= 0 || N <= 0) return STATUS_BYTES;
+  const WsLayout wl = ws_layout(M, N);
+  return M <= 64 ? wl.total : wl.tail_total;
+}
+
+int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* residual, void* y, int M, int N, int K,
+                   int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int activation, void* workspace,
+                   size_t workspace_bytes, int variant, void* stream) {
+  if (!x || !W || !y) return RL_ERR_NULL_POINTER;
+  if (M <= 0 || N <= 0 || K <= 0 || ldx < K || ldw < K || ldy < N || (residual && ldr != 0 && ldr < N))
+    return RL_ERR_BAD_SHAPE;
+  if (activation < RL_ACT_NONE || activation > RL_ACT_SILU) return RL_ERR_BAD_ACTIVATION;
+  if (variant != RL_VARIANT_AUTO && variant != RL_VARIANT_AUTO_WHOLE) return RL_ERR_BAD_VARIANT;
+  if ((K & 7) || (ldx & 7) || (ldw & 7) || !aligned16(x) || !aligned16(W) || (bias && !aligned16(bias)) ||
+      (reinterpret_cast<uintptr_t>(residual) & 1) || (reinterpret_cast<uintptr_t>(y) & 1))
+    return RL_ERR_ALIGNMENT;
+  if (M > 64 && ((ldy & 7) || !aligned16(y))) return RL_ERR_ALIGNMENT;
+  const View vy(y, 2, {{M, ldy}, {N, 1}});
+  if (!disjoint(vy, View(x, 2, {{M, ldx}, {K, 1}})) || !disjoint(vy, View(W, 2, {{N, ldw}, {K, 1}})) ||
+      (bias && !disjoint(vy, View(bias, 2, {{N, 1}}))))
+    return RL_ERR_OVERLAP;
+  if (residual) {
+    const View vr(residual, 2, {{M, ldr}, {N, 1}});
+    if (!vr.same(vy) && !disjoint(vy, vr)) return RL_ERR_OVERLAP;
+  }
+  const WsLayout wl = ws_layout(M, N);
+  if (!workspace || workspace_bytes < (M <= 64 ? wl.total : wl.min_total)) return RL_ERR_WORKSPACE;
+  DeviceInfo di;
+  int rc = device_info(&di);
+  if (rc) return rc;
+  if (di.cc_major != 10) return RL_ERR_UNSUPPORTED_ARCH;
+  PairArgs pa;
+  pa.x = x; pa.W = W; pa.y = y;
+  pa.M = M; pa.N = N; pa.K = K; pa.ldx = ldx; pa.ldw = ldw; pa.ldy = ldy;
+  pa.status = reinterpret_cast<int*>(workspace); pa.ws_bytes = workspace_bytes; pa.tail_off = wl.tail_off; pa.ws_total = wl.tail_total;
+  pa.sync_off = wl.sync_off;
+  pa.sms = di.sms; pa.st = (cudaStream_t)stream;
+  pa.no_norm = true;
+  pa.split_tail = (variant != RL_VARIANT_AUTO_WHOLE);
+  pa.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
+  pa.residual = reinterpret_cast<const __nv_bfloat16*>(residual);
+  pa.ld_res = ldr; pa.act = activation;
+  if (M <= 64) {
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+#define RL_DECODE_LINEAR(MPAD, ST, TW, MINB) \
+  launch_decode<DecodeCfg<MPAD, ST, TW, MINB, false, true>>(x, nullptr, W, y, M, N, K, ldx, ldw, ldy, 0.f, ws, wl, di.sms, \
+                                                            pa.st, nullptr, nullptr, &pa)
+    if (M <= 16) return RL_DECODE_LINEAR(16, RL_DEC16_STAGES, RL_DEC16_TW, RL_DEC16_MINB);
+    if (M <= 32) return RL_DECODE_LINEAR(32, 8, 4, 1);
+    return RL_DECODE_LINEAR(64, 8, 4, 1);
+#undef RL_DECODE_LINEAR
+  }
+  int wide_pairs = 0;
+  if (max_cta_pairs<PairLinearWide>(di.sms, &wide_pairs) == RL_OK && wide_tiles_pay(M, N, K, wide_pairs))
+    return launch_prefill_pair<PairLinearWide>(pa);
+  return launch_prefill_pair<PairLinear>(pa);
+}
+
+int rl_qk_norm_rope_bf16(const void* q, const void* k, const void* q_gamma, const void* k_gamma, const float* table,
+                         const void* positions, int positions_i64, void* q_out, void* k_out, int T, int Hq, int Hk, int D,
+                         int rot, int n_positions, int64_t ld_table, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h,
+                         int64_t qo_t, int64_t qo_h, int64_t ko_t, int64_t ko_h, float eps, int interleaved, void* stream) {
+  if (!q || !k || !table || !positions || !q_out || !k_out) return RL_ERR_NULL_POINTER;
+  if (T <= 0 || Hq <= 0 || Hk <= 0 || D <= 0 || D > 256 || rot <= 0 || rot > D || n_positions < 0 || ld_table < rot ||
+      (long long)Hq + Hk > 65536 || !nonneg({q_t, q_h, k_t, k_h, qo_t, qo_h, ko_t, ko_h}))
+    return RL_ERR_BAD_SHAPE;
+  if ((rot & (interleaved ? 7 : 15)) || (ld_table & 3) || !mult8({D, q_t, q_h, k_t, k_h, qo_t, qo_h, ko_t, ko_h}) ||
+      !aligned16(q) || !aligned16(k) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(table) ||
+      (q_gamma && !aligned16(q_gamma)) || (k_gamma && !aligned16(k_gamma)) ||
+      (reinterpret_cast<uintptr_t>(positions) & (positions_i64 ? 7 : 3)))
+    return RL_ERR_ALIGNMENT;
+  const View vq = head_view(q, T, Hq, D, q_t, q_h), vk = head_view(k, T, Hk, D, k_t, k_h);
+  const View vqo = head_view(q_out, T, Hq, D, qo_t, qo_h), vko = head_view(k_out, T, Hk, D, ko_t, ko_h);
+  const View vt(table, 4, {{n_positions, ld_table}, {rot, 1}}), vp(positions, positions_i64 ? 8 : 4, {{T, 1}});
+  if (vqo.self_overlaps() || vko.self_overlaps() || !disjoint(vqo, vko) || !(vqo.same(vq) || disjoint(vqo, vq)) ||
+      !(vko.same(vk) || disjoint(vko, vk)) || !disjoint(vqo, vk) || !disjoint(vko, vq) || !disjoint(vqo, vt) ||
+      !disjoint(vko, vt) || !disjoint(vqo, vp) || !disjoint(vko, vp))
+    return RL_ERR_OVERLAP;
+  DeviceInfo di;
+  int rc = device_info(&di);
+  if (rc) return rc;
+  if (di.cc_major != 10) return RL_ERR_UNSUPPORTED_ARCH;
+  QkRopeParams p{};
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q); p.k = reinterpret_cast<const __nv_bfloat16*>(k);
+  p.q_gamma = reinterpret_cast<const __nv_bfloat16*>(q_gamma); p.k_gamma = reinterpret_cast<const __nv_bfloat16*>(k_gamma);
+  p.q_out = reinterpret_cast<__nv_bfloat16*>(q_out); p.k_out = reinterpret_cast<__nv_bfloat16*>(k_out);
+  p.table = table; p.positions = positions; p.pos64 = positions_i64; p.n_pos = n_positions;
+  p.T = T; p.Hq = Hq; p.Hk = Hk; p.D = D; p.rot = rot; p.ld_table = ld_table;
+  p.q_t = q_t; p.q_h = q_h; p.k_t = k_t; p.k_h = k_h; p.qo_t = qo_t; p.qo_h = qo_h; p.ko_t = ko_t; p.ko_h = ko_h;
+  p.eps = eps;
+  const int G = lanes_per_row(D);
+  cudaStream_t st = (cudaStream_t)stream;
+#define RL_CALL(g) \
+  (interleaved ? launch_rows(qk_rope_kernel<g, true>, p, T, Hq + Hk, g, st) : launch_rows(qk_rope_kernel<g, false>, p, T, Hq + Hk, g, st))
+  RL_BY_LANES(G, RL_CALL)
+#undef RL_CALL
+}
+
+int rl_kv_cache_write_e4m3(const void* k, const void* v, const void* slots, int slots_i64, void* k_codes, float* k_scale,
+                           void* v_codes, float* v_scale, int T, int H, int D, int num_pages, int page_size, int64_t k_t,
+                           int64_t k_h, int64_t v_t, int64_t v_h, int64_t code_page, int64_t code_token, int64_t code_head,
+                           int64_t scale_page, int64_t scale_token, int64_t scale_head, void* stream) {
+  if (!k || !v || !slots) return RL_ERR_NULL_POINTER;
+  KvWriteParams p{};
+  p.c = KvCache{(uint8_t*)k_codes, (uint8_t*)v_codes, k_scale, v_scale, code_page, code_token, code_head,
+                scale_page, scale_token, scale_head, num_pages, page_size, H, D};
+  int rc = check_cache(p.c);
+  if (rc) return rc;
+  if (T <= 0 || H > 32768 || !nonneg({k_t, k_h, v_t, v_h})) return RL_ERR_BAD_SHAPE;
+  if (!aligned16(k) || !aligned16(v) || !mult8({k_t, k_h, v_t, v_h}) ||
+      (reinterpret_cast<uintptr_t>(slots) & (slots_i64 ? 7 : 3)))
+    return RL_ERR_ALIGNMENT;
+  const View kc = code_view(p.c, k_codes), vc = code_view(p.c, v_codes), ks = scale_view(p.c, k_scale), vs = scale_view(p.c, v_scale);
+  const View vk = head_view(k, T, H, D, k_t, k_h), vv = head_view(v, T, H, D, v_t, v_h), vsl(slots, slots_i64 ? 8 : 4, {{T, 1}});
+  if (kc.self_overlaps() || ks.self_overlaps() || !disjoint(kc, vc) || !disjoint(ks, vs) || !disjoint(kc, ks) ||
+      !disjoint(kc, vs) || !disjoint(vc, ks) || !disjoint(vc, vs))
+    return RL_ERR_OVERLAP;
+  for (const View* c : {&kc, &vc, &ks, &vs})
+    if (!disjoint(*c, vk) || !disjoint(*c, vv) || !disjoint(*c, vsl)) return RL_ERR_OVERLAP;
+  DeviceInfo di;
+  if ((rc = device_info(&di))) return rc;
+  if (di.cc_major != 10) return RL_ERR_UNSUPPORTED_ARCH;
+  p.k = reinterpret_cast<const __nv_bfloat16*>(k); p.v = reinterpret_cast<const __nv_bfloat16*>(v);
+  p.k_t = k_t; p.k_h = k_h; p.v_t = v_t; p.v_h = v_h;
+  p.slots = slots; p.slots64 = slots_i64; p.T = T;
+  const int G = lanes_per_row(D);
+#define RL_CALL(g) launch_rows(kv_write_kernel<g>, p, T, 2 * H, g, (cudaStream_t)stream)
+  RL_BY_LANES(G, RL_CALL)
+#undef RL_CALL
+}
+
+int rl_kv_cache_read_e4m3(const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
+                          const int* page_table, const int* cu_seqlens, void* k_out, void* v_out, int total, int zero_tail,
+                          int B, int max_pages, int64_t ld_pages, int H, int D, int num_pages, int page_size, int64_t code_page,
+                          int64_t code_token, int64_t code_head, int64_t scale_page, int64_t scale_token, int64_t scale_head,
+                          int64_t ko_t, int64_t ko_h, int64_t vo_t, int64_t vo_h, void* stream) {
+  if (!k_out || !v_out || !cu_seqlens || (!page_table && B > 0 && max_pages > 0)) return RL_ERR_NULL_POINTER;
+  KvReadParams p{};
+  p.c = KvCache{(uint8_t*)k_codes, (uint8_t*)v_codes, (float*)k_scale, (float*)v_scale, code_page, code_token, code_head,
+                scale_page, scale_token, scale_head, num_pages, page_size, H, D};
+  int rc = check_cache(p.c);
+  if (rc) return rc;
+  if (total <= 0 || B < 0 || max_pages < 0 || ld_pages < 0 || H > 32768 || !nonneg({ko_t, ko_h, vo_t, vo_h})) return RL_ERR_BAD_SHAPE;
+  if (!aligned16(k_out) || !aligned16(v_out) || !mult8({ko_t, ko_h, vo_t, vo_h}) ||
+      ((reinterpret_cast<uintptr_t>(page_table) | reinterpret_cast<uintptr_t>(cu_seqlens)) & 3))
+    return RL_ERR_ALIGNMENT;
+  const View vko = head_view(k_out, total, H, D, ko_t, ko_h), vvo = head_view(v_out, total, H, D, vo_t, vo_h);
+  const View kc = code_view(p.c, k_codes), vc = code_view(p.c, v_codes), ks = scale_view(p.c, k_scale), vs = scale_view(p.c, v_scale);
+  const View vt(page_table, 4, {{B, ld_pages}, {max_pages, 1}}), vcu(cu_seqlens, 4, {{(int64_t)B + 1, 1}});
+  if (vko.self_overlaps() || vvo.self_overlaps() || !disjoint(vko, vvo)) return RL_ERR_OVERLAP;
+  for (const View* o : {&vko, &vvo})
+    for (const View* i : {&kc, &vc, &ks, &vs, &vt, &vcu})
+      if (!disjoint(*o, *i)) return RL_ERR_OVERLAP;
+  DeviceInfo di;
+  if ((rc = device_info(&di))) return rc;
+  if (di.cc_major != 10) return RL_ERR_UNSUPPORTED_ARCH;
+  p.pages = page_table; p.ld_pages = ld_pages; p.cu = cu_seqlens; p.B = B; p.max_pages = max_pages;
+  p.total = total; p.zero_tail = zero_tail;
+  p.k_out = reinterpret_cast<__nv_bfloat16*>(k_out); p.v_out = reinterpret_cast<__nv_bfloat16*>(v_out);
+  p.ko_t = ko_t; p.ko_h = ko_h; p.vo_t = vo_t; p.vo_h = vo_h;
+  const int G = lanes_per_row(D);
+#define RL_CALL(g) launch_rows(kv_read_kernel<g>, p, total, 2 * H, g, (cudaStream_t)stream)
+  RL_BY_LANES(G, RL_CALL)
+#undef RL_CALL
+}
+
+int rl_take_index_status(int* detail) {
+  int h[4] = {0};
+  cudaError_t e = cudaMemcpyFromSymbol(h, g_index_status, sizeof(h));
+  if (e == cudaSuccess && h[0] != 0) {
+    const int zero[4] = {0};
+    e = cudaMemcpyToSymbol(g_index_status, zero, sizeof(zero));
+  }
+  if (e != cudaSuccess) return cuda_err(e);
+  if (detail)
+    for (int i = 0; i < 4; ++i) detail[i] = h[i];
+  return h[0] == 0 ? RL_OK : RL_ERR_BAD_INDEX;
 }
 
 int rl_selftest_wait_timeout(void* workspace, size_t workspace_bytes, unsigned long long limit_ns, void* stream) {

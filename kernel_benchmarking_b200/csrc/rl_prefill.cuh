@@ -44,6 +44,12 @@ struct PrefillParams {
   unsigned* round_words;
   unsigned round_epoch;    // 20 bits, different for every launch
   unsigned round_wait_ns;
+  // Pair kernels with the linear layer's epilogue (PairCfg::EPI): y = act(x W^T + bias) + residual
+  const __nv_bfloat16* bias;      // [N], 16-byte aligned, or nullptr
+  const __nv_bfloat16* residual;  // [M, N] with leading dimension ld_res, or nullptr; may be the output itself
+  long long ld_res;
+  int res_vec;                    // rows of `residual` start on 16-byte boundaries
+  int act;                        // Activation
 };
 
 // Row statistics on their own: rstd[m] = rsqrt(mean_k x[m,k]^2 + eps).  One warp per token row, 16-byte

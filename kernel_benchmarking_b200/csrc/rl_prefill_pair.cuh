@@ -30,12 +30,13 @@
 //   rsfull[a]   local        row sums of squares written               transform -> own epilogue
 //   rsfree[a]   local        row sums consumed                         epilogue -> own transform warps
 #pragma once
+#include "rl_epilogue.cuh"
 #include "rl_prefill.cuh"
 
 namespace rl {
 
 template <int BN_, int NACC_, int STAGES_, int ASLOTS_, int TG_, int AMODE_, bool PRESTATS_ = false, bool SWIGLU_ = false,
-          bool FP8_ = false>
+          bool FP8_ = false, bool EPI_ = false>
 struct PairCfg {
   static constexpr int BN = BN_, NACC = NACC_, STAGES = STAGES_, ASLOTS = ASLOTS_, TG = TG_, AMODE = AMODE_;
   // PRESTATS: 1/rms per token comes from rowstats_kernel; the transform warps only fold gamma
@@ -50,6 +51,10 @@ struct PairCfg {
   // scales), k-blocks of 128 elements (the same 128 bytes per tile row), kind::f8f6f4 MMAs, and the epilogue
   // multiplies by row_scale[m] * w_scale[n].
   static constexpr bool FP8 = FP8_;
+  // EPI: the linear layer's epilogue (bias, activation, residual) in place of the norm's row scale
+  static constexpr bool EPI = EPI_;
+  static_assert(!EPI_ || (AMODE_ == A_SS_DIRECT && PRESTATS_ && !SWIGLU_ && !FP8_ && NACC_ == 2),
+                "linear epilogue: transform-free bf16, two accumulators");
   static constexpr int KBW = FP8_ ? 128 : 64;  // elements per k-block
   // WIDE (BN = 512): one tile is two MMA-wide column halves that share the activation tile - every x byte brought
   // in from L2 feeds twice the math (the measured upper bound of that saving at the power cap: +7 to +9 %).  The
@@ -137,7 +142,7 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   constexpr bool TS = (Cfg::AMODE == A_TS_FOLD);
   constexpr bool PRESTATS = Cfg::PRESTATS;
   constexpr bool SWIGLU = Cfg::SWIGLU;
-  constexpr bool FP8 = Cfg::FP8, XFORM = Cfg::XFORM, WIDE = Cfg::WIDE;
+  constexpr bool FP8 = Cfg::FP8, XFORM = Cfg::XFORM, WIDE = Cfg::WIDE, EPI = Cfg::EPI;
   constexpr int KBW = Cfg::KBW;
   // k-split tail tiles: 1/rms must come from outside (a slice sees only part of a row) and the epilogue is plain
   constexpr bool TAIL = PRESTATS && !SWIGLU && (BN == 256 || BN == 512);
@@ -497,6 +502,24 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
             o[j] = pack_bf16x2(__uint_as_float(v[2 * j]) * r, __uint_as_float(v[2 * j + 1]) * r);
         }
       };
+      // EPI: 16 columns of the bias, and of this thread's row of the residual, from column n of y
+      [[maybe_unused]] auto load_bias16 = [&](int n, uint32_t (&w)[8]) {
+        if (p.bias == nullptr) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = 0u;
+        } else {
+          load16_bf16(p.bias + n, n, p.N, true, w);
+        }
+      };
+      [[maybe_unused]] auto load_res16 = [&](int n, uint32_t (&w)[8]) {
+        const int m = mt * 256 + (int)rank * 128 + row;
+        if (p.residual == nullptr || m >= p.M) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = 0u;
+        } else {
+          load16_bf16(p.residual + (size_t)m * p.ld_res + n, n, p.N, p.res_vec != 0, w);
+        }
+      };
       // write 64 columns (two 16-word halves) of this thread's row into a swizzled staging tile
       auto sts64 = [&](uint8_t* stage, const uint32_t (&lo)[16], const uint32_t (&hi)[16]) {
 #pragma unroll
@@ -614,15 +637,22 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                   ++b;
                 }
               }
+              if constexpr (EPI) {
+                uint32_t rw[8], bw[8];
+                load_res16(nt * BN + (c_lo + c) * 64 + qq * 16, rw);
+                load_bias16(nt * BN + (c_lo + c) * 64 + qq * 16, bw);
+                epilogue16(a, bw, rw, p.act, &o[qq >> 1][(qq & 1) * 8]);
+              } else {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                float s0 = r, s1 = r;
-                if constexpr (FP8) {
-                  const float2 ws2 = *reinterpret_cast<const float2*>(wc_tile + (c_lo + c) * 64 + qq * 16 + 2 * j);
-                  s0 *= ws2.x;
-                  s1 *= ws2.y;
+                for (int j = 0; j < 8; ++j) {
+                  float s0 = r, s1 = r;
+                  if constexpr (FP8) {
+                    const float2 ws2 = *reinterpret_cast<const float2*>(wc_tile + (c_lo + c) * 64 + qq * 16 + 2 * j);
+                    s0 *= ws2.x;
+                    s1 *= ws2.y;
+                  }
+                  o[qq >> 1][(qq & 1) * 8 + j] = pack_bf16x2(a[2 * j] * s0, a[2 * j + 1] * s1);
                 }
-                o[qq >> 1][(qq & 1) * 8 + j] = pack_bf16x2(a[2 * j] * s0, a[2 * j + 1] * s1);
               }
             }
             sts64(stage, o[0], o[1]);
@@ -783,8 +813,22 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
             if (lane == 0) mbar_arrive_cluster(lead_tempty0 + 8u * (WIDE ? (c > 3 ? 1 : 0) : acc));
           }
           uint32_t lo[16], hi[16];
-          cvt32(v0, lo, c * 64);
-          cvt32(v1, hi, c * 64 + 32);
+          if constexpr (EPI) {
+#pragma unroll
+            for (int qq = 0; qq < 4; ++qq) {
+              const uint32_t(&v)[32] = (qq < 2) ? v0 : v1;
+              uint32_t rw[8], bw[8];
+              load_res16(nt * BN + c * 64 + qq * 16, rw);
+              load_bias16(nt * BN + c * 64 + qq * 16, bw);
+              float z[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(v[(qq & 1) * 16 + j]);
+              epilogue16(z, bw, rw, p.act, (qq < 2 ? lo : hi) + (qq & 1) * 8);
+            }
+          } else {
+            cvt32(v0, lo, c * 64);
+            cvt32(v1, hi, c * 64 + 32);
+          }
           sts64(stage, lo, hi);
           fence_proxy_async_smem();
           named_bar_sync(2, 128);

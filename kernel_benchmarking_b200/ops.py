@@ -8,6 +8,7 @@ top of the C ABI; PyTorch only supplies device memory and the current stream.
 from __future__ import annotations
 
 import ctypes
+import weakref
 from typing import Optional
 
 import torch
@@ -15,6 +16,9 @@ import torch
 from . import _lib
 
 _workspaces: dict = {}
+_own_workspaces: dict = {}   # id -> weak reference: what linear_workspace handed out
+_index_devices: set = set()  # devices on which an operator that takes positions, slots or pages has run
+_CLEAN_BYTES = 256 + 65536   # status block and tile counters: the part of a workspace that starts from zero
 
 
 def _stream_ptr(device: Optional[torch.device] = None) -> int:
@@ -236,6 +240,77 @@ def lora_linear(a: torch.Tensor, b: torch.Tensor, lA: torch.Tensor, lB: torch.Te
     return out
 
 
+def linear_workspace(M: int, N: int, device: Optional[torch.device] = None) -> torch.Tensor:
+    """Scratch for `linear(..., workspace=...)` calls of up to M tokens and N channels (M <= 64 and M > 64 lay theirs out
+    differently: ask with the M of the call).  For calls captured into CUDA graphs: a workspace of one's own is zeroed
+    here, once, and not on every replay.  Calls that share it must not overlap on the device."""
+    ws = torch.zeros(_lib.load().rl_linear_workspace_bytes(M, N), dtype=torch.uint8, device=device or "cuda")
+    key = id(ws)
+    _own_workspaces[key] = weakref.ref(ws, lambda _: _own_workspaces.pop(key, None))
+    return ws
+
+
+def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: Optional[str] = None,
+           residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+           workspace: Optional[torch.Tensor] = None, variant: str = "auto") -> torch.Tensor:
+    """activation(x [M, K] @ W [N, K].t() + bias [N]) + residual [M, N], all bf16, in one kernel: fp32 from the product to
+    the one rounding of the result.  The projection behind an attention or an MLP, added to the residual stream.
+
+    `activation`: None, "relu", "gelu" (erf), "gelu_tanh" or "silu".  `residual` may be `out` itself (an update in
+    place); `out` may share no other memory with the inputs.  Up to 64 tokens run the weight-streaming kernel, more the
+    tensor-core tiles.  `variant="auto_whole"` on streams that run concurrently (see `rmsnorm_linear`).
+
+    Scratch: one workspace per device and stream, as for the other operators.  A call that is being captured into a CUDA
+    graph takes one of its own from the graph's memory and clears it on every replay, so graphs share none; a
+    `linear_workspace` passed in saves that step."""
+    _check_matrix("x", x, torch.bfloat16)
+    _check_matrix("W", W, torch.bfloat16)
+    M, K = x.shape
+    N, K2 = W.shape
+    if K2 != K or W.device != x.device:
+        raise ValueError(f"x is [M, {K}]: W must be [N, {K}] on its device, got {tuple(W.shape)} on {W.device}")
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.dtype != torch.bfloat16 or bias.device != x.device
+                             or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"bias must be a contiguous bf16 vector of length N={N} on x's device")
+    if residual is not None:
+        _check_matrix("residual", residual, torch.bfloat16)
+        if residual.shape != (M, N) or residual.device != x.device:
+            raise ValueError(f"residual must be [{M}, {N}] on x's device, got {tuple(residual.shape)} on {residual.device}")
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"activation must be one of {[a for a in _lib.ACTIVATIONS if a]} or None, got {activation!r}")
+    if variant not in ("auto", "auto_whole"):
+        raise ValueError(f"variant must be 'auto' or 'auto_whole', got {variant!r}")
+    if out is None:
+        ldy = (N + 7) // 8 * 8
+        out = torch.empty((M, ldy), dtype=torch.bfloat16, device=x.device)
+        if ldy != N:
+            out = out[:, :N]
+    else:
+        _check_out(out, M, N, x)
+    if M == 0 or N == 0:
+        return out
+    lib = _lib.load()
+    with _on_device(x.device):
+        stream = _stream_ptr(x.device)
+        nbytes = lib.rl_linear_workspace_bytes(M, N)
+        if workspace is not None:
+            if (not isinstance(workspace, torch.Tensor) or workspace.device != x.device or workspace.dtype != torch.uint8
+                    or not workspace.is_contiguous() or workspace.numel() < nbytes):
+                raise ValueError(f"workspace must be at least {nbytes} contiguous bytes on x's device (linear_workspace)")
+            ws = workspace
+        elif torch.cuda.is_current_stream_capturing():
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            _lib.check(lib.rl_workspace_init(ws.data_ptr(), _CLEAN_BYTES, stream), "rl_workspace_init")
+        else:
+            ws = _workspace(x.device, nbytes, stream)
+        rc = lib.rl_linear_bf16(x.data_ptr(), W.data_ptr(), None if bias is None else bias.data_ptr(),
+                                None if residual is None else residual.data_ptr(), out.data_ptr(), M, N, K, x.stride(0),
+                                W.stride(0), 0 if residual is None else residual.stride(0), out.stride(0),
+                                _lib.ACTIVATIONS[activation], ws.data_ptr(), ws.numel(), _lib.VARIANTS[variant], stream)
+    _lib.check(rc, "rl_linear_bf16")
+    return out
+
+
 def quantize_rows_e4m3(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-6):
     """First kernel of the FP8 path on its own: returns (q [M, K] float8_e4m3fn, row_scale [M] fp32) with
     q = e4m3(x * gamma * 448 / amax_row) and row_scale = rsqrt(mean x^2 + eps) * amax_row / 448."""
@@ -272,14 +347,16 @@ def row_stats(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-6,
 
 def check_status(device: Optional[torch.device] = None) -> None:
     """Synchronise and raise if any kernel launched through this module recorded a device-side
-    timeout.  Kept out of `rmsnorm_linear` so the hot call never synchronises.
+    timeout, or met a position, slot or page outside its table.  Kept out of `rmsnorm_linear` so the hot call never synchronises.
 
     A kernel that gave up a wait may leave tile counters of its workspace non-zero, and every later call on
     that workspace would then be wrong: the workspace is cleared again before the error is raised, so the
     caller can go on after handling it."""
     lib = _lib.load()
     first_error = None
-    for (dev, stream), ws in list(_workspaces.items()):
+    own = [w for w in (ref() for ref in list(_own_workspaces.values())) if w is not None]
+    held = [(dev, stream, ws) for (dev, stream), ws in list(_workspaces.items())]
+    for dev, stream, ws in held + [(w.device.index, None, w) for w in own]:
         if device is not None and torch.device(device).index not in (None, dev):
             continue
         detail = (ctypes.c_int * 8)()
@@ -291,5 +368,16 @@ def check_status(device: Optional[torch.device] = None) -> None:
                 torch.cuda.synchronize()
                 if first_error is None:
                     first_error = f"rmsnorm_linear: {_lib.error_string(rc)}; detail={list(detail)}"
+    for dev in list(_index_devices):
+        if device is not None and torch.device(device).index not in (None, dev):
+            continue
+        detail = (ctypes.c_int * 4)()
+        with torch.cuda.device(dev):
+            torch.cuda.synchronize()
+            rc = lib.rl_take_index_status(detail)
+        if rc != _lib.RL_OK and first_error is None:
+            kind = {1: "position", 2: "slot", 3: "page"}.get(detail[0], "index")
+            first_error = (f"{_lib.error_string(rc)}: {kind} {(detail[2] & 0xffffffff) | (detail[3] << 32)}, "
+                           f"row {detail[1]} of the call, cuda:{dev}")
     if first_error is not None:
         raise RuntimeError(first_error)
