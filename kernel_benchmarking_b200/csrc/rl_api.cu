@@ -704,22 +704,23 @@ bool disjoint(const View& a, const View& b, int i = 0, int j = 0, int64_t shift 
   return false;
 }
 
-// A row kernel's launch: `rows` rows of 8-channel chunks per token, one warp per (token, part).
-// Rows of D channels take G lanes, 32 / G rows per step.
+// How the rows of `tokens` tokens are dealt to warps: every token has `groups` groups of 32 / G rows, a warp takes `steps`
+// of them.  As many as leave 24 warps for every SM - each then has several loads in flight and makes what it needs per
+// token once -, one where there are few rows and only latency counts.
 inline int lanes_per_row(int D) {
-  int g = 2;
-  while (g * 8 < D) g *= 2;
+  int g = 1;
+  while (g * 16 < D) g *= 2;
   return g;
 }
-template <class Params, class Kernel>
-int launch_rows(Kernel kernel, Params& p, int tokens, int rows, int G, cudaStream_t st) {
-  const int R = 32 / G;
-  const int groups = (rows + R - 1) / R;
-  p.steps = 1;
-  p.parts = (groups + p.steps - 1) / p.steps;
-  const long long blocks = ((long long)tokens * p.parts + 3) / 4;
+inline int pick_steps(int tokens, int groups, int sms) {
+  const long long n = (long long)tokens * groups / (24LL * sms);
+  return (int)std::max(1LL, std::min<long long>({n, groups, 16}));
+}
+template <class Params>
+int launch_rows(void (*kernel)(Params), const Params& p, cudaStream_t st) {
+  const long long blocks = ((long long)p.T * p.parts + 3) / 4;
   if (blocks > 0x7fffffffLL) return RL_ERR_BAD_SHAPE;
-  // a programmatic dependent: the kernel touches no global memory before griddepcontrol.wait
+  // a programmatic dependent: the kernels touch no global memory before griddepcontrol.wait
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)blocks);
   lc.blockDim = dim3(128);
@@ -734,11 +735,11 @@ int launch_rows(Kernel kernel, Params& p, int tokens, int rows, int G, cudaStrea
 }
 #define RL_BY_LANES(G, CALL)        \
   switch (G) {                      \
+    case 1: return CALL(1);         \
     case 2: return CALL(2);         \
     case 4: return CALL(4);         \
     case 8: return CALL(8);         \
-    case 16: return CALL(16);       \
-    default: return CALL(32);       \
+    default: return CALL(16);       \
   }
 
 inline bool mult8(std::initializer_list<int64_t> v) {
@@ -1176,10 +1177,15 @@ int rl_qk_norm_rope_bf16(const void* q, const void* k, const void* q_gamma, cons
   p.T = T; p.Hq = Hq; p.Hk = Hk; p.D = D; p.rot = rot; p.ld_table = ld_table;
   p.q_t = q_t; p.q_h = q_h; p.k_t = k_t; p.k_h = k_h; p.qo_t = qo_t; p.qo_h = qo_h; p.ko_t = ko_t; p.ko_h = ko_h;
   p.eps = eps;
-  const int G = lanes_per_row(D);
+  const int G = lanes_per_row(D), R = 32 / G;
+  const int q_groups = (Hq + R - 1) / R, k_groups = (Hk + R - 1) / R;
+  p.steps = pick_steps(T, q_groups + k_groups, di.sms);
+  p.q_parts = (q_groups + p.steps - 1) / p.steps;
+  p.parts = p.q_parts + (k_groups + p.steps - 1) / p.steps;
   cudaStream_t st = (cudaStream_t)stream;
-#define RL_CALL(g) \
-  (interleaved ? launch_rows(qk_rope_kernel<g, true>, p, T, Hq + Hk, g, st) : launch_rows(qk_rope_kernel<g, false>, p, T, Hq + Hk, g, st))
+  // (a head of one lane turns inside it: rot is 16 there, or the pairs are neighbours)
+#define RL_CALL(g) launch_rows(interleaved ? qk_rope_kernel<g, MATE_NEIGHBOUR> : rot == 16 * g ? qk_rope_kernel<g, MATE_OTHER_CHUNK> \
+                                                                                             : qk_rope_kernel<g, (g == 1 ? MATE_OTHER_CHUNK : MATE_ANY)>, p, st)
   RL_BY_LANES(G, RL_CALL)
 #undef RL_CALL
 }
@@ -1211,8 +1217,10 @@ int rl_kv_cache_write_e4m3(const void* k, const void* v, const void* slots, int 
   p.k = reinterpret_cast<const __nv_bfloat16*>(k); p.v = reinterpret_cast<const __nv_bfloat16*>(v);
   p.k_t = k_t; p.k_h = k_h; p.v_t = v_t; p.v_h = v_h;
   p.slots = slots; p.slots64 = slots_i64; p.T = T;
-  const int G = lanes_per_row(D);
-#define RL_CALL(g) launch_rows(kv_write_kernel<g>, p, T, 2 * H, g, (cudaStream_t)stream)
+  const int G = lanes_per_row(D), groups = 2 * ((H + 32 / G - 1) / (32 / G));
+  p.steps = pick_steps(T, groups, di.sms);
+  p.parts = (groups + p.steps - 1) / p.steps;
+#define RL_CALL(g) launch_rows(kv_write_kernel<g>, p, (cudaStream_t)stream)
   RL_BY_LANES(G, RL_CALL)
 #undef RL_CALL
 }
@@ -1243,11 +1251,13 @@ int rl_kv_cache_read_e4m3(const void* k_codes, const float* k_scale, const void*
   if ((rc = device_info(&di))) return rc;
   if (di.cc_major != 10) return RL_ERR_UNSUPPORTED_ARCH;
   p.pages = page_table; p.ld_pages = ld_pages; p.cu = cu_seqlens; p.B = B; p.max_pages = max_pages;
-  p.total = total; p.zero_tail = zero_tail;
+  p.T = total; p.zero_tail = zero_tail;
   p.k_out = reinterpret_cast<__nv_bfloat16*>(k_out); p.v_out = reinterpret_cast<__nv_bfloat16*>(v_out);
   p.ko_t = ko_t; p.ko_h = ko_h; p.vo_t = vo_t; p.vo_h = vo_h;
-  const int G = lanes_per_row(D);
-#define RL_CALL(g) launch_rows(kv_read_kernel<g>, p, total, 2 * H, g, (cudaStream_t)stream)
+  const int G = lanes_per_row(D), groups = 2 * ((H + 32 / G - 1) / (32 / G));
+  p.steps = pick_steps(total, groups, di.sms);
+  p.parts = (groups + p.steps - 1) / p.steps;
+#define RL_CALL(g) launch_rows(kv_read_kernel<g>, p, (cudaStream_t)stream)
   RL_BY_LANES(G, RL_CALL)
 #undef RL_CALL
 }

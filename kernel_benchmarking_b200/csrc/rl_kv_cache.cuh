@@ -34,39 +34,22 @@ struct KvWriteParams {
 // a quotient that is no midpoint is at least 2^-13 of itself away from one, while x * inv is off by at most 2^-23.
 // Rounding the product to 18 bits first puts the midpoints back in their place and moves nothing across one.
 __device__ __forceinline__ uint2 e4m3_codes(const uint32_t (&xs)[4], float inv) {
+  const uint64_t inv2 = pack2(inv, inv), split = pack2(65.0f, 65.0f), minus = pack2(-1.0f, -1.0f);
   uint32_t code[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float q[2] = {bf16lo(xs[i]) * inv, bf16hi(xs[i]) * inv};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float t = __fmul_rn(q[j], 65.0f);  // Veltkamp's splitting: 24 - 6 bits
-      q[j] = __fsub_rn(t, __fsub_rn(t, q[j]));
-    }
-    code[i] = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint64_t q = mul2(widen2(xs[i]), inv2);
+    const uint64_t t = mul2(q, split);                       // Veltkamp's splitting, 24 - 6 bits: t - (t - q), each
+    const float2 v = unpack2(fma2(fma2(q, minus, t), minus, t));  // difference rounded once
+    code[i] = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
   }
   return make_uint2(code[0] | (code[1] << 16), code[2] | (code[3] << 16));
-}
-
-// largest |x| of eight packed bf16 over the lanes of a row, NaN left out
-template <int G>
-__device__ __forceinline__ float row_amax(const uint32_t (&xs)[4]) {
-  __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&xs[i])));
-  uint32_t u = *reinterpret_cast<uint32_t*>(&m);
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) {
-    const uint32_t v = __shfl_xor_sync(0xffffffffu, u, o);
-    m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&v));
-    u = *reinterpret_cast<uint32_t*>(&m);
-  }
-  return fmaxf(bf16lo(u), bf16hi(u));
 }
 
 template <int G>
 __global__ void __launch_bounds__(128) kv_write_kernel(const KvWriteParams p) {
   constexpr int R = 32 / G;
+  constexpr int U = 2;  // groups whose loads are in flight together
   launch_dependents();
   grid_dependency_wait();
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -82,21 +65,53 @@ __global__ void __launch_bounds__(128) kv_write_kernel(const KvWriteParams p) {
     return;
   }
   const long long code_at = page * p.c.c_page + off * p.c.c_off, scale_at = page * p.c.s_page + off * p.c.s_off;
-  const bool have = c * 8 < p.c.D;
-  for (int s = 0; s < p.steps; ++s) {
-    const int h = (part * p.steps + s) * R + lane / G;  // key heads, then value heads
-    const bool is_k = h < p.c.H, row = h < 2 * p.c.H;
-    const int hh = is_k ? h : h - p.c.H;
-    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (row && have)
-      u = *reinterpret_cast<const uint4*>((is_k ? p.k + (size_t)t * p.k_t + (size_t)hh * p.k_h
-                                                : p.v + (size_t)t * p.v_t + (size_t)hh * p.v_h) + c * 8);
-    const uint32_t xs[4] = {u.x, u.y, u.z, u.w};
-    const float a = fmaxf(row_amax<G>(xs), 0x1p-100f);
-    const uint2 codes = e4m3_codes(xs, 448.0f / a);
-    if (row && have)
-      *reinterpret_cast<uint2*>((is_k ? p.c.k_codes : p.c.v_codes) + code_at + (long long)hh * p.c.c_head + c * 8) = codes;
-    if (row && c == 0) (is_k ? p.c.k_scale : p.c.v_scale)[scale_at + (long long)hh * p.c.s_head] = a / 448.0f;
+  const int k_groups = (p.c.H + R - 1) / R;  // the key heads' groups, then as many of the value heads
+  const int g0 = part * p.steps, g1 = min(g0 + p.steps, 2 * k_groups);
+#pragma unroll 1
+  for (int g = g0; g < g1; g += U) {
+    uint32_t x[U][2][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool is_k = g + u < k_groups;
+      const int h = (is_k ? g + u : g + u - k_groups) * R + lane / G;
+      const __nv_bfloat16* src = is_k ? p.k + (size_t)t * p.k_t + h * p.k_h : p.v + (size_t)t * p.v_t + h * p.v_h;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int ch = c + j * G;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (g + u < g1 && h < p.c.H && ch * 8 < p.c.D) v = *reinterpret_cast<const uint4*>(src + ch * 8);
+        x[u][j][0] = v.x; x[u][j][1] = v.y; x[u][j][2] = v.z; x[u][j][3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool is_k = g + u < k_groups;
+      const int h = (is_k ? g + u : g + u - k_groups) * R + lane / G;
+      // largest |x| of the row, NaN left out
+      __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&x[u][j][i])));
+      uint32_t mu = *reinterpret_cast<uint32_t*>(&m);
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mu, o);
+        m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&mu), *reinterpret_cast<const __nv_bfloat162*>(&other));
+        mu = *reinterpret_cast<uint32_t*>(&m);
+      }
+      const float a = fmaxf(fmaxf(bf16lo(mu), bf16hi(mu)), 0x1p-100f);
+      const float inv = 448.0f / a;
+      if (g + u < g1 && h < p.c.H) {
+        uint8_t* dst = (is_k ? p.c.k_codes : p.c.v_codes) + code_at + h * p.c.c_head;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int ch = c + j * G;
+          if (ch * 8 < p.c.D) *reinterpret_cast<uint2*>(dst + ch * 8) = e4m3_codes(x[u][j], inv);
+        }
+        if (c == 0) (is_k ? p.c.k_scale : p.c.v_scale)[scale_at + h * p.c.s_head] = a / 448.0f;
+      }
+    }
   }
 }
 
@@ -105,7 +120,7 @@ struct KvReadParams {
   const int* pages;  // [B, max_pages], leading dimension ld_pages
   long long ld_pages;
   const int* cu;     // [B + 1]: sequence b's tokens are rows cu[b] .. cu[b+1] - 1 of the output
-  int B, max_pages, total, zero_tail, parts, steps;
+  int B, max_pages, T, zero_tail, parts, steps;  // T: rows of the output
   __nv_bfloat16 *k_out, *v_out;
   long long ko_t, ko_h, vo_t, vo_h;
 };
@@ -134,12 +149,13 @@ __device__ __forceinline__ uint32_t dequant2(uint32_t codes, float scale) {
 template <int G>
 __global__ void __launch_bounds__(128) kv_read_kernel(const KvReadParams p) {
   constexpr int R = 32 / G;
+  constexpr int U = 4;  // groups whose loads are in flight together
   launch_dependents();
   grid_dependency_wait();
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, c = lane & (G - 1);
   const int i = (int)(w / p.parts), part = (int)(w - (long long)i * p.parts);
-  if (i >= p.total) return;
+  if (i >= p.T) return;
   const bool held = p.B > 0 && i < p.cu[p.B];
   long long code_at = 0, scale_at = 0;
   if (!held) {
@@ -157,25 +173,41 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const KvReadParams p) {
     code_at = page * p.c.c_page + off * p.c.c_off;
     scale_at = page * p.c.s_page + off * p.c.s_off;
   }
-  const bool have = c * 8 < p.c.D;
-  for (int s = 0; s < p.steps; ++s) {
-    const int h = (part * p.steps + s) * R + lane / G;
-    const bool is_k = h < p.c.H;
-    const int hh = is_k ? h : h - p.c.H;
-    if (h >= 2 * p.c.H || !have) continue;
-    uint32_t o[4] = {0u, 0u, 0u, 0u};
-    if (held) {
-      const float scale = (is_k ? p.c.k_scale : p.c.v_scale)[scale_at + (long long)hh * p.c.s_head];
-      const uint2 u =
-          *reinterpret_cast<const uint2*>((is_k ? p.c.k_codes : p.c.v_codes) + code_at + (long long)hh * p.c.c_head + c * 8);
-      o[0] = dequant2(u.x & 0xffffu, scale);
-      o[1] = dequant2(u.x >> 16, scale);
-      o[2] = dequant2(u.y & 0xffffu, scale);
-      o[3] = dequant2(u.y >> 16, scale);
+  const int k_groups = (p.c.H + R - 1) / R;
+  const int g0 = part * p.steps, g1 = min(g0 + p.steps, 2 * k_groups);
+#pragma unroll 1
+  for (int g = g0; g < g1; g += U) {
+    uint2 code[U][2];
+    float scale[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool is_k = g + u < k_groups;
+      const int h = (is_k ? g + u : g + u - k_groups) * R + lane / G;
+      const bool row = held && g + u < g1 && h < p.c.H;
+      scale[u] = row ? (is_k ? p.c.k_scale : p.c.v_scale)[scale_at + h * p.c.s_head] : 0.f;
+      const uint8_t* src = (is_k ? p.c.k_codes : p.c.v_codes) + code_at + h * p.c.c_head;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int ch = c + j * G;
+        code[u][j] = (row && ch * 8 < p.c.D) ? *reinterpret_cast<const uint2*>(src + ch * 8) : make_uint2(0u, 0u);
+      }
     }
-    *reinterpret_cast<uint4*>((is_k ? p.k_out + (size_t)i * p.ko_t + (size_t)hh * p.ko_h
-                                    : p.v_out + (size_t)i * p.vo_t + (size_t)hh * p.vo_h) + c * 8) =
-        make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool is_k = g + u < k_groups;
+      const int h = (is_k ? g + u : g + u - k_groups) * R + lane / G;
+      if (g + u >= g1 || h >= p.c.H) continue;
+      __nv_bfloat16* dst = is_k ? p.k_out + (size_t)i * p.ko_t + h * p.ko_h : p.v_out + (size_t)i * p.vo_t + h * p.vo_h;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int ch = c + j * G;
+        const uint2 q = code[u][j];
+        if (ch * 8 < p.c.D)
+          *reinterpret_cast<uint4*>(dst + ch * 8) =
+              make_uint4(dequant2(q.x & 0xffffu, scale[u]), dequant2(q.x >> 16, scale[u]), dequant2(q.y & 0xffffu, scale[u]),
+                         dequant2(q.y >> 16, scale[u]));
+      }
+    }
   }
 }
 

@@ -1,8 +1,10 @@
 // What the per-head row kernels (rl_qk_rope.cuh, rl_kv_cache.cuh) share: the record of a bad index, and how a warp
 // lays the rows of one token over its lanes.
 //
-// A row is the D channels of one head of one token (D a multiple of 8, at most 256).  G lanes hold it, G the power of
-// two from D / 8 up (at least 2), eight channels (16 bytes of bf16) each; a warp takes 32 / G rows of the same token at a time.
+// A row is the D channels of one head of one token (D a multiple of 8, at most 256), in chunks of eight channels (16
+// bytes of bf16).  G lanes hold it, G the power of two from D / 16 up: lane c has chunks c and c + G, so that a row's
+// loads and stores are contiguous over the lanes, and a warp takes 32 / G rows of the same token at a time.  (One chunk
+// per lane spends twice the reductions, roots and divisions per row; these kernels issue nearly as long as they load.)
 #pragma once
 #include "rl_ptx.cuh"
 
@@ -27,12 +29,27 @@ __device__ __forceinline__ long long load_index(const void* p, int i, int is64) 
   return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
 }
 
-// sum over the G neighbouring lanes that hold a row (G a power of two)
-template <int G>
-__device__ __forceinline__ float row_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// packed fp32 pairs (sm_100), each half rounded to nearest like the scalar operation
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
 }
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t widen2(uint32_t bf16x2) { return pack2(bf16lo(bf16x2), bf16hi(bf16x2)); }
 
 }  // namespace rl

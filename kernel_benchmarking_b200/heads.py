@@ -10,12 +10,13 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _index_devices, _on_device, _stream_ptr
-
-_INDEX_TYPES = (torch.int64, torch.int32)
+from .ops import _index_devices, _raw_stream
 
 
-def _check_heads(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
+# The checks sit on the path of every decode step, whose kernels run for a few microseconds: each call makes them as one
+# plain condition first and looks for what is wrong, and the words for it, only when that fails.
+
+def _explain_heads(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> None:
     """[tokens, heads, channels] bf16 on the GPU, channels contiguous; the strides of tokens and heads are free."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -25,14 +26,34 @@ def _check_heads(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None
         raise ValueError(f"{name} must be torch.bfloat16, got {t.dtype}")
     if t.dim() != 3 or t.stride(2) != 1:
         raise ValueError(f"{name} must be [tokens, heads, channels] with contiguous channels, got {tuple(t.shape)}")
-    if like is not None and t.device != like.device:
-        raise ValueError(f"{name} must be on {like.device}, got {t.device}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
 
 
-def _check_index(name: str, t: torch.Tensor, n: int, like: torch.Tensor, types=_INDEX_TYPES) -> None:
-    if (not isinstance(t, torch.Tensor) or t.dtype not in types or t.dim() != 1 or t.shape[0] != n
-            or t.device != like.device or (n > 1 and t.stride(0) != 1)):
-        raise ValueError(f"{name} must be a contiguous vector of {n} {' or '.join(str(x) for x in types)} on {like.device}")
+def _heads_ok(t: torch.Tensor, dev: int) -> bool:
+    return (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.get_device() == dev and t.dim() == 3
+            and t.stride(2) == 1)
+
+
+def _index_ok(t: torch.Tensor, n: int, dev: int) -> bool:
+    """A contiguous vector of n int64 or int32."""
+    return (isinstance(t, torch.Tensor) and (t.dtype is torch.int64 or t.dtype is torch.int32) and t.get_device() == dev
+            and t.dim() == 1 and t.shape[0] == n and (t.stride(0) == 1 or n <= 1))
+
+
+def _gamma_ok(g: Optional[torch.Tensor], D: int, dev: int) -> bool:
+    return g is None or (isinstance(g, torch.Tensor) and g.dtype is torch.bfloat16 and g.get_device() == dev
+                         and g.shape == (D,) and (g.stride(0) == 1 or D <= 1))
+
+
+def _call(dev: int, fn, *args) -> int:
+    """The C function with the device's current stream behind the arguments, on that device."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    return rc
 
 
 def rope_table(positions: int, rotary_dim: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:
@@ -56,48 +77,69 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: Optional[torch.Tenso
     `positions` [T] int64 or int32; one outside the table leaves its token's rows unwritten and `check_status` raises.
     D a multiple of 8 up to 256, rotary_dim of 16 (interleaved: 8).  `out`: a pair of tensors to write, q and k
     themselves for an update in place; they may share no other memory with the inputs or each other."""
-    _check_heads("q", q)
-    _check_heads("k", k, q)
+    dev = q.get_device() if isinstance(q, torch.Tensor) and q.is_cuda else None
+    if dev is None or not (_heads_ok(q, dev) and _heads_ok(k, dev)):
+        _explain_heads("q", q)
+        _explain_heads("k", k, q.device)
     T, Hq, D = q.shape
-    Hk = k.shape[1]
-    if k.shape[0] != T or k.shape[2] != D:
+    Tk, Hk, Dk = k.shape
+    if Tk != T or Dk != D:
         raise ValueError(f"q is [{T}, {Hq}, {D}]: k must be [{T}, Hk, {D}], got {tuple(k.shape)}")
-    for name, g in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
-        if g is not None and (not isinstance(g, torch.Tensor) or g.dtype != torch.bfloat16 or g.device != q.device
-                              or g.shape != (D,) or (D > 1 and g.stride(0) != 1)):
-            raise ValueError(f"{name} must be a contiguous bf16 vector of length D={D} on q's device")
-    if (not isinstance(table, torch.Tensor) or table.dtype != torch.float32 or table.dim() != 2 or table.device != q.device
-            or table.stride(1) != 1):
+    if not (_gamma_ok(q_gamma, D, dev) and _gamma_ok(k_gamma, D, dev)):
+        raise ValueError(f"q_gamma and k_gamma must be contiguous bf16 vectors of length D={D} on q's device")
+    if (not isinstance(table, torch.Tensor) or table.dtype is not torch.float32 or table.dim() != 2
+            or table.get_device() != dev or table.stride(1) != 1):
         raise ValueError("table must be [positions, rotary_dim] fp32, row-major, on q's device")
-    _check_index("positions", positions, T, q)
+    if not _index_ok(positions, T, dev):
+        raise ValueError(f"positions must be a contiguous vector of {T} int64 or int32 on q's device")
     if out is None:
-        qo = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
-        ko = torch.empty((T, Hk, D), dtype=torch.bfloat16, device=q.device)
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
         qo, ko = out
-        _check_heads("out[0]", qo, q)
-        _check_heads("out[1]", ko, q)
+        if not (_heads_ok(qo, dev) and _heads_ok(ko, dev)):
+            _explain_heads("out[0]", qo, q.device)
+            _explain_heads("out[1]", ko, q.device)
         if qo.shape != q.shape or ko.shape != k.shape:
             raise ValueError(f"out must be {tuple(q.shape)} and {tuple(k.shape)}, got {tuple(qo.shape)} and {tuple(ko.shape)}")
     if T == 0:
         return qo, ko
-    with _on_device(q.device):
-        rc = _lib.load().rl_qk_norm_rope_bf16(
-            q.data_ptr(), k.data_ptr(), None if q_gamma is None else q_gamma.data_ptr(),
-            None if k_gamma is None else k_gamma.data_ptr(), table.data_ptr(), positions.data_ptr(),
-            positions.dtype == torch.int64, qo.data_ptr(), ko.data_ptr(), T, Hq, Hk, D, table.shape[1], table.shape[0],
-            table.stride(0), q.stride(0), q.stride(1), k.stride(0), k.stride(1), qo.stride(0), qo.stride(1), ko.stride(0),
-            ko.stride(1), eps, interleaved, _stream_ptr(q.device))
-    _lib.check(rc, "rl_qk_norm_rope_bf16")
-    _index_devices.add(q.device.index)
+    P, rot = table.shape
+    q_t, q_h, _ = q.stride()
+    k_t, k_h, _ = k.stride()
+    qo_t, qo_h, _ = qo.stride()
+    ko_t, ko_h, _ = ko.stride()
+    rc = _call(dev, _lib.load().rl_qk_norm_rope_bf16,
+               q.data_ptr(), k.data_ptr(), None if q_gamma is None else q_gamma.data_ptr(),
+               None if k_gamma is None else k_gamma.data_ptr(), table.data_ptr(), positions.data_ptr(),
+               positions.dtype is torch.int64, qo.data_ptr(), ko.data_ptr(), T, Hq, Hk, D, rot, P, table.stride(0), q_t, q_h,
+               k_t, k_h, qo_t, qo_h, ko_t, ko_h, eps, interleaved)
+    if rc:
+        _lib.check(rc, "rl_qk_norm_rope_bf16")
+    _index_devices.add(dev)
     return qo, ko
 
 
-def _check_cache(k_codes, k_scale, v_codes, v_scale) -> None:
-    for name, t, dtype, nd in (("k_codes", k_codes, torch.float8_e4m3fn, 4), ("v_codes", v_codes, torch.float8_e4m3fn, 4),
-                               ("k_scale", k_scale, torch.float32, 3), ("v_scale", v_scale, torch.float32, 3)):
+def _cache_ok(k_codes, k_scale, v_codes, v_scale, dev: int) -> bool:
+    shape, strides = k_codes.shape, k_codes.stride()
+    return (k_codes.dtype is torch.float8_e4m3fn and v_codes.dtype is torch.float8_e4m3fn and k_scale.dtype is torch.float32
+            and v_scale.dtype is torch.float32 and v_codes.get_device() == dev and k_scale.get_device() == dev
+            and v_scale.get_device() == dev and len(shape) == 4 and strides[3] == 1 and v_codes.shape == shape
+            and v_codes.stride() == strides and k_scale.shape == shape[:3] and v_scale.shape == shape[:3]
+            and v_scale.stride() == k_scale.stride())
+
+
+def _check_cache(k_codes, k_scale, v_codes, v_scale) -> int:
+    """Returns the cache's device index."""
+    named = (("k_codes", k_codes), ("k_scale", k_scale), ("v_codes", v_codes), ("v_scale", v_scale))
+    for name, t in named:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
+    dev = k_codes.get_device()
+    if dev >= 0 and _cache_ok(k_codes, k_scale, v_codes, v_scale, dev):
+        return dev
+    for name, t in named:
+        dtype, nd = (torch.float8_e4m3fn, 4) if name.endswith("codes") else (torch.float32, 3)
         if not t.is_cuda:
             raise ValueError(f"{name} must be a CUDA tensor (this operator has no CPU path)")
         if t.dtype != dtype or t.dim() != nd or t.device != k_codes.device:
@@ -106,8 +148,7 @@ def _check_cache(k_codes, k_scale, v_codes, v_scale) -> None:
         raise ValueError("the codes' channels must be contiguous")
     if v_codes.shape != k_codes.shape or v_codes.stride() != k_codes.stride():
         raise ValueError("v_codes must have the shape and strides of k_codes")
-    if k_scale.shape != k_codes.shape[:3] or v_scale.shape != k_scale.shape or v_scale.stride() != k_scale.stride():
-        raise ValueError(f"k_scale and v_scale must both be {tuple(k_codes.shape[:3])}, with the same strides")
+    raise ValueError(f"k_scale and v_scale must both be {tuple(k_codes.shape[:3])}, with the same strides")
 
 
 def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch.Tensor, k_scale: torch.Tensor,
@@ -119,24 +160,29 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_code
     channels, the same for keys and values.  `slots` [T] int64 or int32: page * page_size + place in the page.  Negative:
     a padding token, left out.  Beyond the cache: left out, and `check_status` raises.  The slots of one call must differ.
     A NaN stays NaN; a row with an infinity reads back as NaN throughout.  D a multiple of 8 up to 256."""
-    _check_cache(k_codes, k_scale, v_codes, v_scale)
-    _check_heads("k", k, k_codes)
-    _check_heads("v", v, k_codes)
+    dev = _check_cache(k_codes, k_scale, v_codes, v_scale)
+    if not (_heads_ok(k, dev) and _heads_ok(v, dev)):
+        _explain_heads("k", k, k_codes.device)
+        _explain_heads("v", v, k_codes.device)
     T, H, D = k.shape
-    pages, page_size = k_codes.shape[:2]
-    if v.shape != k.shape or k_codes.shape[2:] != (H, D):
-        raise ValueError(f"k and v must be [T, {k_codes.shape[2]}, {k_codes.shape[3]}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    _check_index("slots", slots, T, k)
+    pages, page_size, Hc, Dc = k_codes.shape
+    if v.shape != k.shape or Hc != H or Dc != D:
+        raise ValueError(f"k and v must be [T, {Hc}, {Dc}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if not _index_ok(slots, T, dev):
+        raise ValueError(f"slots must be a contiguous vector of {T} int64 or int32 on the cache's device")
     if T == 0:
         return
-    c, s = k_codes.stride(), k_scale.stride()
-    with _on_device(k.device):
-        rc = _lib.load().rl_kv_cache_write_e4m3(
-            k.data_ptr(), v.data_ptr(), slots.data_ptr(), slots.dtype == torch.int64, k_codes.data_ptr(), k_scale.data_ptr(),
-            v_codes.data_ptr(), v_scale.data_ptr(), T, H, D, pages, page_size, k.stride(0), k.stride(1), v.stride(0),
-            v.stride(1), c[0], c[1], c[2], s[0], s[1], s[2], _stream_ptr(k.device))
-    _lib.check(rc, "rl_kv_cache_write_e4m3")
-    _index_devices.add(k.device.index)
+    c_page, c_off, c_head, _ = k_codes.stride()
+    s_page, s_off, s_head = k_scale.stride()
+    k_t, k_h, _ = k.stride()
+    v_t, v_h, _ = v.stride()
+    rc = _call(dev, _lib.load().rl_kv_cache_write_e4m3,
+               k.data_ptr(), v.data_ptr(), slots.data_ptr(), slots.dtype is torch.int64, k_codes.data_ptr(),
+               k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), T, H, D, pages, page_size, k_t, k_h, v_t, v_h,
+               c_page, c_off, c_head, s_page, s_off, s_head)
+    if rc:
+        _lib.check(rc, "rl_kv_cache_write_e4m3")
+    _index_devices.add(dev)
 
 
 def kv_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
@@ -149,33 +195,37 @@ def kv_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.T
     `total` is the caller's: rows from cu_seqlens[B] on are zero in a fresh output and left as they are in `out`,
     tokens beyond `total` are not read.  A page outside the cache (or a sequence longer than its table row) leaves the
     row as it is, unspecified in a fresh output, and `check_status` raises."""
-    _check_cache(k_codes, k_scale, v_codes, v_scale)
+    dev = _check_cache(k_codes, k_scale, v_codes, v_scale)
     pages, page_size, H, D = k_codes.shape
-    if (not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or page_table.dim() != 2
-            or page_table.device != k_codes.device or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+    if (not isinstance(page_table, torch.Tensor) or page_table.dtype is not torch.int32 or page_table.dim() != 2
+            or page_table.get_device() != dev or (page_table.stride(1) != 1 and page_table.shape[1] > 1)):
         raise ValueError("page_table must be [B, max_pages] int32, row-major, on the cache's device")
-    B = page_table.shape[0]
-    _check_index("cu_seqlens", cu_seqlens, B + 1, k_codes, (torch.int32,))
+    B, max_pages = page_table.shape
+    if not _index_ok(cu_seqlens, B + 1, dev) or cu_seqlens.dtype is not torch.int32:
+        raise ValueError(f"cu_seqlens must be a contiguous vector of {B + 1} int32 on the cache's device")
     if total < 0:
         raise ValueError("total must not be negative")
     if out is None:
-        ko = torch.empty((total, H, D), dtype=torch.bfloat16, device=k_codes.device)
-        vo = torch.empty((total, H, D), dtype=torch.bfloat16, device=k_codes.device)
+        ko = k_codes.new_empty((total, H, D), dtype=torch.bfloat16)
+        vo = k_codes.new_empty((total, H, D), dtype=torch.bfloat16)
     else:
         ko, vo = out
-        _check_heads("out[0]", ko, k_codes)
-        _check_heads("out[1]", vo, k_codes)
+        if not (_heads_ok(ko, dev) and _heads_ok(vo, dev)):
+            _explain_heads("out[0]", ko, k_codes.device)
+            _explain_heads("out[1]", vo, k_codes.device)
         if ko.shape != (total, H, D) or vo.shape != ko.shape:
             raise ValueError(f"out must be two tensors [{total}, {H}, {D}], got {tuple(ko.shape)} and {tuple(vo.shape)}")
     if total == 0:
         return ko, vo
-    c, s = k_codes.stride(), k_scale.stride()
-    with _on_device(k_codes.device):
-        rc = _lib.load().rl_kv_cache_read_e4m3(
-            k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
-            cu_seqlens.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, out is None, B, page_table.shape[1],
-            page_table.stride(0), H, D, pages, page_size, c[0], c[1], c[2], s[0], s[1], s[2], ko.stride(0), ko.stride(1),
-            vo.stride(0), vo.stride(1), _stream_ptr(k_codes.device))
-    _lib.check(rc, "rl_kv_cache_read_e4m3")
-    _index_devices.add(k_codes.device.index)
+    c_page, c_off, c_head, _ = k_codes.stride()
+    s_page, s_off, s_head = k_scale.stride()
+    ko_t, ko_h, _ = ko.stride()
+    vo_t, vo_h, _ = vo.stride()
+    rc = _call(dev, _lib.load().rl_kv_cache_read_e4m3,
+               k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
+               cu_seqlens.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, out is None, B, max_pages, page_table.stride(0),
+               H, D, pages, page_size, c_page, c_off, c_head, s_page, s_off, s_head, ko_t, ko_h, vo_t, vo_h)
+    if rc:
+        _lib.check(rc, "rl_kv_cache_read_e4m3")
+    _index_devices.add(dev)
     return ko, vo

@@ -8,6 +8,7 @@ top of the C ABI; PyTorch only supplies device memory and the current stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import weakref
 from typing import Optional
 
@@ -21,11 +22,15 @@ _index_devices: set = set()  # devices on which an operator that takes positions
 _CLEAN_BYTES = 256 + 65536   # status block and tile counters: the part of a workspace that starts from zero
 
 
-def _stream_ptr(device: Optional[torch.device] = None) -> int:
-    """Raw handle of torch's current stream on `device` (the fast C accessor when torch has it)."""
-    idx = torch.cuda.current_device() if device is None or device.index is None else device.index
+def _raw_stream(idx: int) -> int:
+    """Raw handle of torch's current stream on device `idx` (the fast C accessor when torch has it)."""
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return raw(idx) if raw is not None else torch.cuda.current_stream(idx).cuda_stream
+
+
+def _stream_ptr(device: Optional[torch.device] = None) -> int:
+    """Raw handle of torch's current stream on `device`."""
+    return _raw_stream(torch.cuda.current_device() if device is None or device.index is None else device.index)
 
 
 class _on_device:
@@ -240,6 +245,16 @@ def lora_linear(a: torch.Tensor, b: torch.Tensor, lA: torch.Tensor, lB: torch.Te
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace_bytes(M: int, N: int) -> int:
+    return _lib.load().rl_linear_workspace_bytes(M, N)
+
+
+def _matrix_ok(t: torch.Tensor, dev: int) -> bool:
+    return (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.get_device() == dev and t.dim() == 2
+            and t.stride(1) == 1)
+
+
 def linear_workspace(M: int, N: int, device: Optional[torch.device] = None) -> torch.Tensor:
     """Scratch for `linear(..., workspace=...)` calls of up to M tokens and N channels (M <= 64 and M > 64 lay theirs out
     differently: ask with the M of the call).  For calls captured into CUDA graphs: a workspace of one's own is zeroed
@@ -263,52 +278,65 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
     Scratch: one workspace per device and stream, as for the other operators.  A call that is being captured into a CUDA
     graph takes one of its own from the graph's memory and clears it on every replay, so graphs share none; a
     `linear_workspace` passed in saves that step."""
-    _check_matrix("x", x, torch.bfloat16)
-    _check_matrix("W", W, torch.bfloat16)
+    # one plain condition on the path of every decode step; what is wrong is looked for only when it fails
+    dev = x.get_device() if isinstance(x, torch.Tensor) and x.is_cuda else None
+    if dev is None or not (_matrix_ok(x, dev) and _matrix_ok(W, dev) and (residual is None or _matrix_ok(residual, dev))):
+        _check_matrix("x", x, torch.bfloat16)
+        _check_matrix("W", W, torch.bfloat16)
+        if residual is not None:
+            _check_matrix("residual", residual, torch.bfloat16)
+        raise ValueError("x, W and residual must be on one device")
     M, K = x.shape
     N, K2 = W.shape
-    if K2 != K or W.device != x.device:
-        raise ValueError(f"x is [M, {K}]: W must be [N, {K}] on its device, got {tuple(W.shape)} on {W.device}")
-    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.dtype != torch.bfloat16 or bias.device != x.device
-                             or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
+    if K2 != K:
+        raise ValueError(f"x is [M, {K}]: W must be [N, {K}], got {tuple(W.shape)}")
+    if bias is not None and not (isinstance(bias, torch.Tensor) and bias.dtype is torch.bfloat16 and bias.get_device() == dev
+                                 and bias.shape == (N,) and (bias.stride(0) == 1 or N <= 1)):
         raise ValueError(f"bias must be a contiguous bf16 vector of length N={N} on x's device")
-    if residual is not None:
-        _check_matrix("residual", residual, torch.bfloat16)
-        if residual.shape != (M, N) or residual.device != x.device:
-            raise ValueError(f"residual must be [{M}, {N}] on x's device, got {tuple(residual.shape)} on {residual.device}")
-    if activation not in _lib.ACTIVATIONS:
+    if residual is not None and residual.shape != (M, N):
+        raise ValueError(f"residual must be [{M}, {N}], got {tuple(residual.shape)}")
+    act = _lib.ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {[a for a in _lib.ACTIVATIONS if a]} or None, got {activation!r}")
     if variant not in ("auto", "auto_whole"):
         raise ValueError(f"variant must be 'auto' or 'auto_whole', got {variant!r}")
     if out is None:
         ldy = (N + 7) // 8 * 8
-        out = torch.empty((M, ldy), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((M, ldy))
         if ldy != N:
             out = out[:, :N]
     else:
         _check_out(out, M, N, x)
     if M == 0 or N == 0:
         return out
+    nbytes = _linear_workspace_bytes(M, N)
+    if workspace is not None and not (isinstance(workspace, torch.Tensor) and workspace.get_device() == dev
+                                      and workspace.dtype is torch.uint8 and workspace.is_contiguous()
+                                      and workspace.numel() >= nbytes):
+        raise ValueError(f"workspace must be at least {nbytes} contiguous bytes on x's device (linear_workspace)")
+    if dev == torch.cuda.current_device():
+        rc = _launch_linear(dev, x, W, bias, residual, out, M, N, K, act, workspace, nbytes, variant)
+    else:
+        with torch.cuda.device(dev):
+            rc = _launch_linear(dev, x, W, bias, residual, out, M, N, K, act, workspace, nbytes, variant)
+    if rc:
+        _lib.check(rc, "rl_linear_bf16")
+    return out
+
+
+def _launch_linear(dev, x, W, bias, residual, out, M, N, K, act, ws, nbytes, variant) -> int:
     lib = _lib.load()
-    with _on_device(x.device):
-        stream = _stream_ptr(x.device)
-        nbytes = lib.rl_linear_workspace_bytes(M, N)
-        if workspace is not None:
-            if (not isinstance(workspace, torch.Tensor) or workspace.device != x.device or workspace.dtype != torch.uint8
-                    or not workspace.is_contiguous() or workspace.numel() < nbytes):
-                raise ValueError(f"workspace must be at least {nbytes} contiguous bytes on x's device (linear_workspace)")
-            ws = workspace
-        elif torch.cuda.is_current_stream_capturing():
+    stream = _raw_stream(dev)
+    if ws is None:
+        if torch.cuda.is_current_stream_capturing():
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
             _lib.check(lib.rl_workspace_init(ws.data_ptr(), _CLEAN_BYTES, stream), "rl_workspace_init")
         else:
             ws = _workspace(x.device, nbytes, stream)
-        rc = lib.rl_linear_bf16(x.data_ptr(), W.data_ptr(), None if bias is None else bias.data_ptr(),
-                                None if residual is None else residual.data_ptr(), out.data_ptr(), M, N, K, x.stride(0),
-                                W.stride(0), 0 if residual is None else residual.stride(0), out.stride(0),
-                                _lib.ACTIVATIONS[activation], ws.data_ptr(), ws.numel(), _lib.VARIANTS[variant], stream)
-    _lib.check(rc, "rl_linear_bf16")
-    return out
+    return lib.rl_linear_bf16(x.data_ptr(), W.data_ptr(), None if bias is None else bias.data_ptr(),
+                              None if residual is None else residual.data_ptr(), out.data_ptr(), M, N, K, x.stride(0),
+                              W.stride(0), 0 if residual is None else residual.stride(0), out.stride(0), act, ws.data_ptr(),
+                              ws.numel(), _lib.VARIANTS[variant], stream)
 
 
 def quantize_rows_e4m3(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-6):
