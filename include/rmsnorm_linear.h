@@ -46,7 +46,7 @@ enum {
   RL_ERR_TENSOR_MAP = -8,       /* the driver rejected a TMA descriptor */
   RL_ERR_DEVICE_TIMEOUT = -9,   /* a bounded wait inside a kernel ran out (reported by rl_read_status) */
   RL_ERR_STATIC_SCRATCH = -10,  /* rl_rmsnorm_linear_bf16_noalloc: the shape needs more scratch than the built-in buffer */
-  RL_ERR_BAD_INDEX = -11,       /* a kernel met a position, slot or page outside its table (reported by rl_take_index_status) */
+  RL_ERR_BAD_INDEX = -11,       /* a kernel met a position, slot or page outside its table (reported by rl_take_device_status) */
   RL_ERR_OVERLAP = -12,         /* an output shares memory with an input, another output or itself */
   RL_ERR_BAD_ACTIVATION = -13,  /* unknown RL_ACT_* code */
   RL_ERR_CUDA = -1000           /* RL_ERR_CUDA - cudaError_t of the failing runtime call */
@@ -223,12 +223,14 @@ int rl_lora_linear_bf16(const void* a, const void* b, const void* xa, const void
  * be y itself (same pointer and leading dimension), any other sharing of y's memory is RL_ERR_OVERLAP.
  *   K, ldx, ldw multiples of 8; x, W, bias 16-byte aligned; for M > 64 ldy a multiple of 8 and y 16-byte aligned.
  *   residual may have any leading dimension from N up, or 0: one row for every token (16-byte aligned rows read fastest).
- *   M <= 64 runs the weight-streaming kernel of rl_rmsnorm_linear_bf16 without its norm, larger M the CTA-pair tiles.
- *   workspace: rl_linear_workspace_bytes(M, N) bytes, as for every operator here zeroed once, one per stream (for
- *   M > 64 one that ends before the k-split blocks is accepted; every tile is then computed whole).
+ *   Few tokens or few tiles run a kernel that shares every tile's k-loop among the CTAs of a cluster and needs no
+ *   workspace (rl_linear_workspace_bytes is 0; a wait that ran out is reported by rl_take_device_status); the others run
+ *   the CTA-pair tiles.
+ *   workspace: rl_linear_workspace_bytes(M, N, K) bytes, as for every operator here zeroed once, one per stream (one that
+ *   ends before the k-split blocks is accepted; every tile is then computed whole).
  *   variant: RL_VARIANT_AUTO or RL_VARIANT_AUTO_WHOLE (see Concurrency above).
  * No reference counterpart beyond its plain GEMM (demo/new_profiling/rmsnorm_linear_new.py:29-31). */
-size_t rl_linear_workspace_bytes(int M, int N);
+size_t rl_linear_workspace_bytes(int M, int N, int K);
 int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* residual, void* y, int M, int N, int K,
                    int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int activation,
                    void* workspace, size_t workspace_bytes, int variant, void* stream);
@@ -243,7 +245,7 @@ int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* r
  *   rot / 2 sines of each position.  positions [T] int32, or int64 with positions_i64.
  *   D a multiple of 8, at most 256; rot a multiple of 16 (interleaved: 8), at most D; strides multiples of 8 elements,
  *   ld_table of 4; pointers 16-byte aligned.
- *   A position outside the table: that token's rows are not written, and rl_take_index_status reports it.
+ *   A position outside the table: that token's rows are not written, and rl_take_device_status reports it.
  * No workspace.  No reference counterpart. */
 int rl_qk_norm_rope_bf16(const void* q, const void* k, const void* q_gamma, const void* k_gamma, const float* table,
                          const void* positions, int positions_i64, void* q_out, void* k_out, int T, int Hq, int Hk, int D,
@@ -256,7 +258,7 @@ int rl_qk_norm_rope_bf16(const void* q, const void* k, const void* q_gamma, cons
  *   k, v [T, H, D] bf16, strides (token, head) in elements.  codes [num_pages, page_size, H, D] bytes, scales
  *   [num_pages, page_size, H] fp32, strides (page, token, head) in elements, the same for keys and values.
  *   slots [T] int32, or int64 with slots_i64: page * page_size + place in the page.  A negative slot is a padding token
- *   and left out; one beyond the cache is left out and reported by rl_take_index_status.  The slots of one call
+ *   and left out; one beyond the cache is left out and reported by rl_take_device_status.  The slots of one call
  *   must differ: where two tokens name one slot, its codes and scale may come from either.
  *   D a multiple of 8, at most 256; strides of k, v and the codes multiples of 8; k, v 16-byte, codes 8-byte aligned.
  * No workspace.  No reference counterpart. */
@@ -270,7 +272,7 @@ int rl_kv_cache_write_e4m3(const void* k, const void* v, const void* slots, int 
  *   page_table [B, max_pages] int32, leading dimension ld_pages; cu_seqlens [B + 1] int32, not decreasing, from 0.
  *   Rows from cu_seqlens[B] on are left as they are, or zeroed with zero_tail; tokens beyond `total` are not read.
  *   A page outside the cache, or a sequence longer than its table row: the row is left as it is and
- *   rl_take_index_status reports it.
+ *   rl_take_device_status reports it.
  * Cache arguments and alignments as for rl_kv_cache_write_e4m3.  No workspace.  No reference counterpart. */
 int rl_kv_cache_read_e4m3(const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
                           const int* page_table, const int* cu_seqlens, void* k_out, void* v_out, int total, int zero_tail,
@@ -278,11 +280,12 @@ int rl_kv_cache_read_e4m3(const void* k_codes, const float* k_scale, const void*
                           int64_t code_token, int64_t code_head, int64_t scale_page, int64_t scale_token, int64_t scale_head,
                           int64_t ko_t, int64_t ko_h, int64_t vo_t, int64_t vo_h, void* stream);
 
-/* The first position, slot or page that a kernel of the three functions above found outside its table on the current
- * device since this was last called (it clears the record; call it outside the hot loop, with the streams
- * synchronised).  RL_OK or RL_ERR_BAD_INDEX; detail, unless NULL, receives 4 ints: 1 position / 2 slot / 3 page, the
- * row of the call, and the index (low and high word).  No reference counterpart. */
-int rl_take_index_status(int* detail);
+/* What the kernels without a workspace recorded on the current device since this was last called (it clears the record;
+ * call it outside the hot loop, with the streams synchronised): the first position, slot or page that a kernel of the
+ * three functions above found outside its table, or a wait inside rl_linear_bf16's cluster kernel that ran out.  RL_OK,
+ * RL_ERR_BAD_INDEX or RL_ERR_DEVICE_TIMEOUT; detail, unless NULL, receives 4 ints: 1 position / 2 slot / 3 page, the row of
+ * the call, and the index (low and high word); or for a wait code, role, barrier, block.  No reference counterpart. */
+int rl_take_device_status(int* detail);
 
 /* Self-test of the kernels' failure detection.  Launches one small CTA that waits on a barrier nothing
  * ever arrives on, with the given limit (<= 1 s); the wait must give up, record RL_ERR_DEVICE_TIMEOUT

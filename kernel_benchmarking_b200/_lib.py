@@ -68,12 +68,12 @@ SYMBOLS = [
     ("rl_rmsnorm_swiglu_bf16", _i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _f, _vp, _sz, _vp]),
     ("rl_gemm_bf16", _i, [_vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _vp, _sz, _vp]),
     ("rl_lora_linear_bf16", _i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
-    ("rl_linear_workspace_bytes", _sz, [_i, _i]),
+    ("rl_linear_workspace_bytes", _sz, [_i, _i, _i]),
     ("rl_linear_bf16", _i, [_vp] * 5 + [_i] * 3 + [_i64] * 4 + [_i, _vp, _sz, _i, _vp]),
     ("rl_qk_norm_rope_bf16", _i, [_vp] * 6 + [_i, _vp, _vp] + [_i] * 6 + [_i64] * 9 + [_f, _i, _vp]),
     ("rl_kv_cache_write_e4m3", _i, [_vp] * 3 + [_i] + [_vp] * 4 + [_i] * 5 + [_i64] * 10 + [_vp]),
     ("rl_kv_cache_read_e4m3", _i, [_vp] * 8 + [_i] * 4 + [_i64] + [_i] * 4 + [_i64] * 10 + [_vp]),
-    ("rl_take_index_status", _i, [ctypes.POINTER(ctypes.c_int)]),
+    ("rl_take_device_status", _i, [ctypes.POINTER(ctypes.c_int)]),
     ("rl_selftest_wait_timeout", _i, [_vp, _sz, ctypes.c_ulonglong, _vp]),
     ("rl_read_status", _i, [_vp, ctypes.POINTER(ctypes.c_int)]),
 ]

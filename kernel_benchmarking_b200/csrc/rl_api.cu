@@ -10,6 +10,7 @@
 
 #include "rl_decode.cuh"
 #include "rl_kv_cache.cuh"
+#include "rl_linear_split.cuh"
 #include "rl_qk_rope.cuh"
 #include "rl_rowquant.cuh"
 #include "rl_prefill.cuh"
@@ -368,7 +369,7 @@ int launch_prefill_pair(const PairArgs& a) {
   if ((rc = make_map(&tw, dt, eb, a.W, K, Cfg::SWIGLU ? 2 * (uint64_t)N : (uint64_t)N, a.ldw, Cfg::KBW,
                      Cfg::WIDE ? 128 : Cfg::BN / 2)))
     return rc;
-  if ((rc = make_map(&ty, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, N, M, a.ldy, 64, 128))) return rc;
+  if ((rc = make_map(&ty, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.y, N, M, a.ldy, 64, Cfg::EPI ? 32 : 128))) return rc;
   if (Cfg::AMODE == A_SS_DIRECT && a.gamma != nullptr && !prescale) return RL_ERR_BAD_VARIANT;
   tx2 = tx;
   tw2 = tw;
@@ -437,8 +438,9 @@ int launch_prefill_pair(const PairArgs& a) {
     p.round_epoch = (++epoch_counter) & 0xfffffu;
     p.round_wait_ns = RL_ROUND_WAIT_NS;
   }
-  if (Cfg::PRESTATS && p.row_rstd != nullptr) {
-    // behind rowstats_kernel (FP8: rowquant_kernel) with programmatic stream serialisation: the GEMM sets up
+  if ((Cfg::PRESTATS && p.row_rstd != nullptr) || Cfg::EPI) {
+    // (the linear layer: a programmatic dependent of whatever runs in front, all of whose threads wait before they touch
+    // global memory.)  The others: behind rowstats_kernel (FP8: rowquant_kernel) with programmatic stream serialisation: the GEMM sets up
     // and, in the bf16 case, streams its tiles while the row statistics are still being computed, and waits only
     // where it first reads them.  Only in that case: rowstats_kernel and rowscale_kernel are normal launches, so
     // everything earlier in the stream (whoever wrote x and W) is complete before they start, and the producer
@@ -478,14 +480,12 @@ using DecodeCfg16 = DecodeCfg<16, RL_DEC16_STAGES, RL_DEC16_TW, RL_DEC16_MINB>;
 template <class Cfg>
 int launch_decode(const void* x, const __nv_bfloat16* gamma, const void* W, void* y, int M, int N, int K,
                   int64_t ldx, int64_t ldw, int64_t ldy, float eps, uint8_t* ws, const WsLayout& wl, int sms,
-                  cudaStream_t st, const float* row_scale = nullptr, const float* w_scale = nullptr,
-                  const PairArgs* epilogue = nullptr) {
+                  cudaStream_t st, const float* row_scale = nullptr, const float* w_scale = nullptr) {
   CUtensorMap tw, tx;
   int rc;
   const CUtensorMapDataType dt = Cfg::FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int eb = Cfg::FP8 ? 1 : 2;
   if (Cfg::FP8 && (!row_scale || !w_scale)) return RL_ERR_NULL_POINTER;
-  if (Cfg::LINEAR && !epilogue) return RL_ERR_BAD_VARIANT;
   if ((rc = make_map(&tw, dt, eb, W, K, N, ldw, Cfg::KBW, 128))) return rc;
   if ((rc = make_map(&tx, dt, eb, x, K, M, ldx, Cfg::KBW, Cfg::MPAD))) return rc;
   DecodeParams p{};
@@ -493,12 +493,6 @@ int launch_decode(const void* x, const __nv_bfloat16* gamma, const void* W, void
   p.gamma = gamma;
   p.row_scale = row_scale;
   p.w_scale = w_scale;
-  if (Cfg::LINEAR) {
-    p.bias = epilogue->bias;
-    p.residual = epilogue->residual;
-    p.ld_res = epilogue->ld_res;
-    p.act = epilogue->act;
-  }
   p.y = reinterpret_cast<__nv_bfloat16*>(y);
   p.ldy = ldy;
   p.n_tiles = (N + 127) / 128;
@@ -534,6 +528,77 @@ int launch_decode(const void* x, const __nv_bfloat16* gamma, const void* W, void
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, decode_kernel<Cfg>, tw, tx, p);
+  return e == cudaSuccess ? RL_OK : cuda_err(e);
+}
+
+// ---- the cluster-split kernel of the linear layer
+struct SplitPlan {
+  int nt, split;  // tokens per tile, CTAs per cluster; nt = 0: the CTA-pair kernel
+};
+// Cluster-split kernel or CTA pairs, and the former's tile and cluster size: the least of what a short model says, in
+// microseconds.  Its figures are fits to measurements of 36 shapes with every tile and cluster size (tokens 1..4096, K
+// 256..14336): 5.5 us for a launch, its pipeline's start and its exchange (2 more for 128-token tiles, 0.25 per part), and
+// the k-blocks at 160 KB/us an SM with two CTAs or more on it, 85 with one.  The pairs: 10 us (8 without an epilogue, 12
+// with everything), and 0.34 per k-block of a round of tiles.  Measured, split against pairs: 128 x 4096 x 4096 13.6 / 20.4
+// us, 512 x 4096 x 4096 21.0 / 23.4, 1024^3 8.4 / 12.6, 1500 x 1536 x 1536 12.9 / 16.0, 4096 x 512 x 256 6.5 / 8.7; the
+// other way round 512 x 4096 x 14336 58 / 53, 1024 x 4096 x 4096 34.7 / 29.9.  Up to 64 tokens it is always the former
+// (against the weight-streaming kernel of the norm: 16 x 4096 x 4096 9.9 / 13.2 us, 64 x 14336 x 4096 23.3 / 32, 64 x
+// 28672 x 4096 42.8 / 45.5).  The plan is arithmetic on the sizes, for the 148 SMs of a B200.
+SplitPlan plan_split(int M, int N, int K) {
+  constexpr int SMS = 148, PAIRS = 74;
+  const int KB = (K + 63) / 64;
+  SplitPlan best{0, 1};
+  double best_us = 1e30;
+  const int nt_first = M <= 16 ? 16 : (M <= 32 ? 32 : 64), nt_last = M <= 64 ? nt_first : 128;
+  for (int nt = nt_first; nt <= nt_last; nt *= 2) {
+    const long long tiles = (long long)((M + nt - 1) / nt) * ((N + 127) / 128);
+    for (int s = 1; s <= 8 && (s == 1 || (tiles * s <= 2 * SMS && KB >= 2 * s)); s *= 2) {
+      const long long ctas = tiles * s, per_sm = (ctas + SMS - 1) / SMS;
+      if (M > 64 && per_sm > 2) break;
+      const double kb_us = (16.0 + nt / 8.0) / (per_sm >= 2 ? 160.0 : 85.0);
+      const double us = 5.5 + (double)per_sm * ((KB + s - 1) / s) * kb_us + 0.25 * s + (nt == 128 ? 2.0 : 0.0);
+      if (us < best_us) { best_us = us; best = SplitPlan{nt, s}; }
+    }
+  }
+  if (M > 64) {
+    const long long tiles = (long long)((M + 255) / 256) * ((N + 255) / 256);
+    if (10.0 + 0.34 * KB * rounds_cost(tiles, PAIRS, KB) < best_us) return SplitPlan{0, 1};
+  }
+  return best;
+}
+
+template <class Cfg>
+int launch_split(const PairArgs& a, int split) {
+  CUtensorMap tw, tx;
+  int rc;
+  if ((rc = make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.W, a.K, a.N, a.ldw, 64, 128))) return rc;
+  if ((rc = make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.x, a.K, a.M, a.ldx, 64, Cfg::NT))) return rc;
+  SplitParams p{};
+  p.M = a.M; p.N = a.N; p.K = a.K;
+  p.token_tiles = (a.M + Cfg::NT - 1) / Cfg::NT;
+  p.split = split; p.act = a.act;
+  p.bias = a.bias; p.residual = a.residual; p.y = reinterpret_cast<__nv_bfloat16*>(a.y);
+  p.ld_res = a.ld_res; p.ldy = a.ldy;
+  p.res_vec = (a.ld_res & 3) == 0 && (reinterpret_cast<uintptr_t>(a.residual) & 7) == 0;
+  p.y_vec = (a.ldy & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7) == 0;
+  const long long blocks = (long long)p.token_tiles * ((a.N + 127) / 128) * split;
+  if (blocks > 0x7fffffffLL) return RL_ERR_BAD_SHAPE;
+  cudaError_t e = set_smem_once(linear_split_kernel<Cfg>, Cfg::SMEM_BYTES, true);
+  if (e != cudaSuccess) return cuda_err(e);
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)blocks);
+  lc.blockDim = dim3(Cfg::THREADS);
+  lc.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  lc.stream = a.st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)split; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  // a programmatic dependent: nothing in global memory is touched before griddepcontrol.wait
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = at;
+  lc.numAttrs = 2;
+  e = cudaLaunchKernelEx(&lc, linear_split_kernel<Cfg>, tw, tx, p);
   return e == cudaSuccess ? RL_OK : cuda_err(e);
 }
 
@@ -1086,10 +1151,9 @@ int rl_lora_linear_bf16(const void* a, const void* b, const void* xa, const void
   return launch_prefill_pair<PairDirect>(pa);
 }
 
-size_t rl_linear_workspace_bytes(int M, int N) {
-  if (M <= 0 || N <= 0) return STATUS_BYTES;
-  const WsLayout wl = ws_layout(M, N);
-  return M <= 64 ? wl.total : wl.tail_total;
+size_t rl_linear_workspace_bytes(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || plan_split(M, N, K).nt != 0) return 0;
+  return ws_layout(M, N).tail_total;
 }
 
 int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* residual, void* y, int M, int N, int K,
@@ -1112,8 +1176,9 @@ int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* r
     const View vr(residual, 2, {{M, ldr}, {N, 1}});
     if (!vr.same(vy) && !disjoint(vy, vr)) return RL_ERR_OVERLAP;
   }
+  const SplitPlan plan = plan_split(M, N, K);
   const WsLayout wl = ws_layout(M, N);
-  if (!workspace || workspace_bytes < (M <= 64 ? wl.total : wl.min_total)) return RL_ERR_WORKSPACE;
+  if (plan.nt == 0 && (!workspace || workspace_bytes < wl.min_total)) return RL_ERR_WORKSPACE;
   DeviceInfo di;
   int rc = device_info(&di);
   if (rc) return rc;
@@ -1129,18 +1194,22 @@ int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* r
   pa.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
   pa.residual = reinterpret_cast<const __nv_bfloat16*>(residual);
   pa.ld_res = ldr; pa.act = activation;
-  if (M <= 64) {
-    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-#define RL_DECODE_LINEAR(MPAD, ST, TW, MINB) \
-  launch_decode<DecodeCfg<MPAD, ST, TW, MINB, false, true>>(x, nullptr, W, y, M, N, K, ldx, ldw, ldy, 0.f, ws, wl, di.sms, \
-                                                            pa.st, nullptr, nullptr, &pa)
-    if (M <= 16) return RL_DECODE_LINEAR(16, RL_DEC16_STAGES, RL_DEC16_TW, RL_DEC16_MINB);
-    if (M <= 32) return RL_DECODE_LINEAR(32, 8, 4, 1);
-    return RL_DECODE_LINEAR(64, 8, 4, 1);
-#undef RL_DECODE_LINEAR
+  if (plan.nt != 0) {
+    switch (plan.nt) {
+      case 16: return launch_split<SplitCfg<16, 6>>(pa, plan.split);
+      case 32: return launch_split<SplitCfg<32, 5>>(pa, plan.split);
+      case 64: return launch_split<SplitCfg<64, 4>>(pa, plan.split);
+      default: return launch_split<SplitCfg<128, 3>>(pa, plan.split);
+    }
   }
+  // The 256 x 512 tiles' epilogue is not hidden behind the next tile's main loop as the 256 x 256 tiles' is.  Measured, it
+  // costs a tile the time of 4 k-blocks, 9 with a residual, 11 with an activation, 16 with both, where the narrow tiles as
+  // a whole are 5 to 8 % slower: 4096 x 14336 x 4096 with everything 388 us narrow, 426 wide (plain GEMM 340), 8192 x 4096
+  // x 14336 768 and 716.
   int wide_pairs = 0;
-  if (max_cta_pairs<PairLinearWide>(di.sms, &wide_pairs) == RL_OK && wide_tiles_pay(M, N, K, wide_pairs))
+  const int KB = (K + 63) / 64;
+  if (KB >= 64 + (residual ? 64 : 0) + (activation != RL_ACT_NONE ? 80 : 0) &&
+      max_cta_pairs<PairLinearWide>(di.sms, &wide_pairs) == RL_OK && wide_tiles_pay(M, N, K, wide_pairs))
     return launch_prefill_pair<PairLinearWide>(pa);
   return launch_prefill_pair<PairLinear>(pa);
 }
@@ -1262,17 +1331,18 @@ int rl_kv_cache_read_e4m3(const void* k_codes, const float* k_scale, const void*
 #undef RL_CALL
 }
 
-int rl_take_index_status(int* detail) {
-  int h[4] = {0};
-  cudaError_t e = cudaMemcpyFromSymbol(h, g_index_status, sizeof(h));
-  if (e == cudaSuccess && h[0] != 0) {
-    const int zero[4] = {0};
-    e = cudaMemcpyToSymbol(g_index_status, zero, sizeof(zero));
-  }
+int rl_take_device_status(int* detail) {
+  int index[4] = {0}, wait[RL_STATUS_INTS] = {0};
+  const int zero[RL_STATUS_INTS] = {0};
+  cudaError_t e = cudaMemcpyFromSymbol(index, g_index_status, sizeof(index));
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(wait, g_wait_status, sizeof(wait));
+  if (e == cudaSuccess && index[0] != 0) e = cudaMemcpyToSymbol(g_index_status, zero, sizeof(index));
+  if (e == cudaSuccess && wait[0] != 0) e = cudaMemcpyToSymbol(g_wait_status, zero, sizeof(wait));
   if (e != cudaSuccess) return cuda_err(e);
+  const int* from = wait[0] != 0 ? wait : index;
   if (detail)
-    for (int i = 0; i < 4; ++i) detail[i] = h[i];
-  return h[0] == 0 ? RL_OK : RL_ERR_BAD_INDEX;
+    for (int i = 0; i < 4; ++i) detail[i] = from[i];
+  return wait[0] != 0 ? RL_ERR_DEVICE_TIMEOUT : (index[0] != 0 ? RL_ERR_BAD_INDEX : RL_OK);
 }
 
 int rl_selftest_wait_timeout(void* workspace, size_t workspace_bytes, unsigned long long limit_ns, void* stream) {

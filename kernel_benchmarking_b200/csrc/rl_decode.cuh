@@ -24,7 +24,6 @@
 // two CTAs per SM (6 stages, 2 transform warps, 256 threads), so that the next launch's CTAs could
 // set up on the free half while this launch drains, measured the same as with one CTA per SM.
 #pragma once
-#include "rl_epilogue.cuh"
 #include "rl_ptx.cuh"
 
 namespace rl {
@@ -46,14 +45,9 @@ struct DecodeParams {
   // FP8 configuration: x is the e4m3 activation matrix from rowquant_kernel, W the e4m3 weights
   const float* row_scale;  // [M] rsqrt(mean x^2 + eps) * amax / 448 per token
   const float* w_scale;    // [N] per-output-channel weight scales
-  // linear configuration: y = act(x W^T + bias) + residual
-  const __nv_bfloat16* bias;      // [N] or nullptr
-  const __nv_bfloat16* residual;  // [M, N] with leading dimension ld_res, or nullptr; may be y itself
-  long long ld_res;
-  int act;                        // Activation
 };
 
-template <int MPAD_, int STAGES_, int TW_ = 4, int MINB_ = 1, bool FP8_ = false, bool LINEAR_ = false>
+template <int MPAD_, int STAGES_, int TW_ = 4, int MINB_ = 1, bool FP8_ = false>
 struct DecodeCfg {
   static constexpr int MPAD = MPAD_, STAGES = STAGES_;
   // FP8: e4m3 weights and per-token e4m3 activations (quantised beforehand by rowquant_kernel), kind::f8f6f4
@@ -61,9 +55,6 @@ struct DecodeCfg {
   // inside the activations and their per-token scale, so the transform warps only pass the tiles on, and the
   // epilogue multiplies by row_scale[m] * w_scale[n].  Half the weight bytes of the bf16 kernel per launch.
   static constexpr bool FP8 = FP8_;
-  // LINEAR: no norm and no gamma - the transform warps pass the tiles on - and the linear layer's epilogue
-  static constexpr bool LINEAR = LINEAR_;
-  static_assert(!(FP8_ && LINEAR_), "the linear configuration is bf16");
   static constexpr int KBW = FP8_ ? 128 : 64;  // elements per k-block
   static constexpr int TW = TW_;      // transform warps; units are dealt to them round-robin
   static constexpr int MINB = MINB_;  // CTAs per SM the kernel is compiled (and sized) for
@@ -137,8 +128,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::MINB)
 decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
               const DecodeParams p) {
   constexpr int MPAD = Cfg::MPAD, STAGES = Cfg::STAGES, NCH = Cfg::NCH, TW = Cfg::TW, KBW = Cfg::KBW;
-  constexpr bool FP8 = Cfg::FP8, LINEAR = Cfg::LINEAR;
-  constexpr bool NORM = !FP8 && !LINEAR;  // sums of squares and gamma belong to this kernel
+  constexpr bool FP8 = Cfg::FP8;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -161,7 +151,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ 
   const int G = (int)gridDim.x, cta = (int)blockIdx.x;
   const int u_begin = sk_begin(cta, p.units_total, G);
   const int u_end = sk_begin(cta + 1, p.units_total, G);
-  const bool has_gamma = NORM && (p.gamma != nullptr);
+  const bool has_gamma = !FP8 && (p.gamma != nullptr);
   const DecodeSegments segs(u_begin, u_end, KB, p.sk_tiles + cta, p.whole_per_cta, G);
 
   // one unit's loads: W tile (streamed once: evict-first), x tile (re-read by every CTA: evict-last), gamma slice
@@ -296,7 +286,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ 
         ok = mbar_wait(bar_full(s), ph, ctl, 2, s, u + i);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (!NORM) {  // nothing to fold and nothing to sum: hand the tile on
+        if (FP8) {  // nothing to fold and nothing to sum: hand the tile on
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_xf(s));
           continue;
@@ -387,13 +377,13 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ 
       if (FP8) wsn = (n < p.N) ? __ldg(p.w_scale + n) : 0.f;
       // one thread per token adds up the transform warps' shares of the sum of squares
       float tot = 0.f;
-      if (!LINEAR && epi_tid < MPAD) {
+      if (epi_tid < MPAD) {
 #pragma unroll
         for (int w = 0; w < TW; ++w) tot += ssq[(w * 2 + acc) * MPAD + epi_tid];
       }
       bool finish = whole;
       if (whole) {
-        if (!LINEAR && epi_tid < MPAD)
+        if (epi_tid < MPAD)
           rvec[epi_tid] = FP8 ? ((epi_tid < p.M) ? __ldg(p.row_scale + epi_tid) : 0.f) : 1.0f / sqrtf(tot * inv_k + p.eps);
         named_bar_sync(1, 128);
       } else {
@@ -401,7 +391,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ 
         float* part = p.partials + (size_t)(cta * 2 + slot) * MPAD * 128;
 #pragma unroll
         for (int m = 0; m < MPAD; ++m) part[m * 128 + n_local] = a[m];
-        if (NORM && epi_tid < MPAD) p.ssq_partials[(cta * 2 + slot) * MPAD + epi_tid] = tot;
+        if (!FP8 && epi_tid < MPAD) p.ssq_partials[(cta * 2 + slot) * MPAD + epi_tid] = tot;
         __threadfence();
         named_bar_sync(1, 128);
         const int first = sk_cta_of_unit(tile * KB, p.units_total, G);
@@ -426,32 +416,17 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ 
             float ld[MPAD];
 #pragma unroll
             for (int m = 0; m < MPAD; ++m) ld[m] = __ldcg(cpart + m * 128 + n_local);
-            if (NORM && epi_tid < MPAD) s2 += __ldcg(p.ssq_partials + (cc * 2 + cslot) * MPAD + epi_tid);
+            if (!FP8 && epi_tid < MPAD) s2 += __ldcg(p.ssq_partials + (cc * 2 + cslot) * MPAD + epi_tid);
 #pragma unroll
             for (int m = 0; m < MPAD; ++m) a[m] += ld[m];
           }
-          if (!LINEAR && epi_tid < MPAD)
+          if (epi_tid < MPAD)
             rvec[epi_tid] = FP8 ? ((epi_tid < p.M) ? __ldg(p.row_scale + epi_tid) : 0.f) : 1.0f / sqrtf(s2 * inv_k + p.eps);
           named_bar_sync(5, 128);
         }
       }
       if (finish) {
-        if constexpr (LINEAR) {
-          if (n < p.N) {
-            const float b = (p.bias != nullptr) ? __bfloat162float(p.bias[n]) : 0.f;
-#pragma unroll
-            for (int m = 0; m < MPAD; ++m) a[m] += b;
-            apply_activation(a, p.act);
-            if (p.residual != nullptr) {
-#pragma unroll
-              for (int m = 0; m < MPAD; ++m)
-                if (m < p.M) a[m] += __bfloat162float(p.residual[(size_t)m * p.ld_res + n]);
-            }
-#pragma unroll
-            for (int m = 0; m < MPAD; ++m)
-              if (m < p.M) p.y[(size_t)m * p.ldy + n] = __float2bfloat16_rn(a[m]);
-          }
-        } else if (n < p.N) {
+        if (n < p.N) {
 #pragma unroll
           for (int m = 0; m < MPAD; ++m)
             if (m < p.M) p.y[(size_t)m * p.ldy + n] = __float2bfloat16_rn(FP8 ? a[m] * rvec[m] * wsn : a[m] * rvec[m]);

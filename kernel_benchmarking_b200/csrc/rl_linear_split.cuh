@@ -1,0 +1,255 @@
+// The linear layer for few tokens or few tiles: y = act(x W^T + bias) + residual with the k-loop of every tile shared by the
+// CTAs of a cluster.
+//
+// Operands are swapped so that the 128-wide UMMA M dimension runs over output channels: A = W tile [128 x 64], B = x tile
+// [NT tokens x 64], D[channel, token] in tensor memory.  The `split` CTAs of a cluster (1, 2, 4 or 8) take one contiguous
+// part of the tile's k-blocks each, leave their fp32 accumulators in their own shared memory, and after one cluster barrier
+// each finishes its share of the tokens: it adds the parts in rank order out of its neighbours' shared memory, so results do
+// not depend on timing, and nothing is exchanged through global memory.  No workspace, no counters, and no CTA waits for
+// one outside its cluster, which the hardware schedules together.
+//
+// Warps: 0 TMA producer, 1 UMMA issuer, then the epilogue's.
+#pragma once
+#include "rl_epilogue.cuh"
+#include "rl_ptx.cuh"
+
+namespace rl {
+
+struct SplitParams {
+  int M, N, K;
+  int token_tiles, split, act;
+  const __nv_bfloat16* bias;      // [N] or nullptr
+  const __nv_bfloat16* residual;  // [M, N] with leading dimension ld_res, or nullptr; may be y itself
+  __nv_bfloat16* y;
+  long long ld_res, ldy;
+  int res_vec, y_vec;             // rows start on 8-byte boundaries
+};
+
+template <int NT_, int STAGES_>
+struct SplitCfg {
+  static constexpr int NT = NT_, STAGES = STAGES_;
+  // epilogue warps: eight halve the time of the wide tiles' epilogues, four cost the short ones less to launch (0.5 us)
+  static constexpr int EPI_WARPS = NT >= 64 ? 8 : 4, THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int W_BYTES = 128 * 64 * 2, X_BYTES = NT * 64 * 2;
+  static constexpr int OFF_W = 0, OFF_X = STAGES * W_BYTES;
+  static constexpr int RING_BYTES = STAGES * (W_BYTES + X_BYTES);
+  static constexpr int OFF_BAR = RING_BYTES;
+  static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 1) * 8;
+  static constexpr int SMEM_BYTES = OFF_MISC + 64 + 1024;
+  static constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
+  static_assert(NT == 16 || NT == 32 || NT == 64 || NT == 128, "tokens per tile");
+  static_assert(NT * 128 * 4 <= RING_BYTES, "the accumulator fits where the operands were");
+};
+
+// where a wait that ran out is recorded (layout of the status block); part of the device image like g_index_status
+static __device__ int g_wait_status[RL_STATUS_INTS];
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+
+// residual of tokens first and first + EW (zeros where there is none)
+template <int EW>
+__device__ __forceinline__ void split_residual(const SplitParams& p, int m0, int n, int first, int last, uint2 (&res)[2]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int tk = first + EW * u;
+    res[u] = make_uint2(0u, 0u);
+    if (tk < last && p.residual != nullptr && n < p.N)
+      res[u] = load4_bf16(p.residual + (size_t)(m0 + tk) * p.ld_res + n, n, p.N, p.res_vec != 0);
+  }
+}
+
+// The tokens first, first + EW, .. below `last` of a tile (EW epilogue warps), four channels per lane: parts in rank order, bias, activation,
+// residual.  Two tokens at a time; `res` comes in with the first two's residual, and the next two's is on its way while
+// these are finished.
+template <int S, int EW>
+__device__ __forceinline__ void split_finish(const SplitParams& p, uint32_t part, int m0, int n, int first, int last,
+                                             const uint32_t (&bias)[2], uint2 (&res)[2]) {
+  uint32_t from[S];
+#pragma unroll
+  for (int r = 0; r < S; ++r) from[r] = mapa_shared(part, (uint32_t)r);
+  for (int t0 = first; t0 < last; t0 += 2 * EW) {
+    float4 v[2][S];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < S; ++r)
+        if (t0 + EW * u < last) v[u][r] = ld_cluster_f4(from[r] + (uint32_t)(t0 + EW * u) * 512u);
+    uint2 next[2];
+    split_residual<EW>(p, m0, n, t0 + 2 * EW, last, next);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int tk = t0 + EW * u;
+      if (tk >= last || n >= p.N) continue;
+      uint64_t z[2] = {pack2(v[u][0].x, v[u][0].y), pack2(v[u][0].z, v[u][0].w)};
+#pragma unroll
+      for (int r = 1; r < S; ++r) {
+        z[0] = add2(z[0], pack2(v[u][r].x, v[u][r].y));
+        z[1] = add2(z[1], pack2(v[u][r].z, v[u][r].w));
+      }
+      const uint32_t rw[2] = {res[u].x, res[u].y};
+      uint32_t o[2];
+      linear_epilogue(z, bias, rw, p.act, o);
+      __nv_bfloat16* dst = p.y + (size_t)(m0 + tk) * p.ldy + n;
+      if (p.y_vec && n + 4 <= p.N) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+      } else {
+        unsigned short* d = reinterpret_cast<unsigned short*>(dst);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < p.N) d[i] = (unsigned short)(o[i >> 1] >> ((i & 1) * 16));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) res[u] = next[u];
+  }
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 2)
+linear_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const SplitParams p) {
+  constexpr int NT = Cfg::NT, STAGES = Cfg::STAGES, EW = Cfg::EPI_WARPS;
+  extern __shared__ uint8_t smem_raw[];
+  // (every CTA of the kernel has the same shared-memory layout, so the aligned base is the same in the whole cluster)
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + Cfg::OFF_BAR;
+  auto bar_full = [&](int s) { return bar0 + 8u * s; };
+  auto bar_empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  const uint32_t bar_acc = bar0 + 8u * (2 * STAGES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_MISC);
+  CtaCtl* ctl = reinterpret_cast<CtaCtl*>(smem + Cfg::OFF_MISC + 16);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = p.split;
+  const int rank = (int)(blockIdx.x % S), tile = (int)(blockIdx.x / S);
+  const int tt = tile % p.token_tiles, ct = tile / p.token_tiles;
+  const int KB = (p.K + 63) >> 6;
+  const int kb0 = (int)((long long)rank * KB / S), kb1 = (int)((long long)(rank + 1) * KB / S);  // never empty: S <= KB
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full(s), 1);
+      mbar_init(bar_empty(s), 1);
+    }
+    mbar_init(bar_acc, 1);
+    ctl->abort = 0;
+    ctl->status = g_wait_status;
+    ctl->limit_ns = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // only now may the next kernel's CTAs come in beside this one: its tensor memory is taken already
+  launch_dependents();
+  grid_dependency_wait();
+
+  const int m0 = tt * NT, n0 = ct * 128;
+  const int tokens = min(NT, p.M - m0);
+  // the tokens this warp will finish (rank's share, from `first` in steps of EW), and what that needs early: the bias of the
+  // lane's four channels and the first tokens' residual
+  const int per = NT / S;
+  const int first = rank * per + (warp - 2), last = min(tokens, (rank + 1) * per);
+  uint2 res[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+  if (warp >= 2) split_residual<EW>(p, m0, n0 + lane * 4, first, last, res);
+  uint32_t bias[2] = {0u, 0u};
+  if (warp >= 2 && p.bias != nullptr && n0 + lane * 4 < p.N) {
+    const uint2 w = load4_bf16(p.bias + n0 + lane * 4, n0 + lane * 4, p.N, true);
+    bias[0] = w.x;
+    bias[1] = w.y;
+  }
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    const uint64_t pol_w = (p.token_tiles == 1) ? l2_policy_evict_first() : l2_policy_evict_last();
+    const uint64_t pol_x = l2_policy_evict_last();
+    int s = 0;
+    uint32_t ph = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(bar_empty(s), ph ^ 1, ctl, 0, STAGES + s, kb)) break;
+      if (elect_one()) {
+        mbar_expect_tx(bar_full(s), Cfg::W_BYTES + Cfg::X_BYTES);
+        tma_load_2d_hint(sbase + Cfg::OFF_W + s * Cfg::W_BYTES, &tm_w, bar_full(s), kb * 64, n0, pol_w);
+        tma_load_2d_hint(sbase + Cfg::OFF_X + s * Cfg::X_BYTES, &tm_x, bar_full(s), kb * 64, m0, pol_x);
+      }
+      __syncwarp();
+      if (++s == STAGES) { s = 0; ph ^= 1; }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ UMMA issuer
+    constexpr uint32_t idesc = make_idesc(128, NT, 1, 1);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(bar_full(s), ph, ctl, 1, s, kb)) { ok = false; break; }
+      tc_fence_after();
+      const uint64_t adesc = make_sw128_kmajor_desc(sbase + Cfg::OFF_W + s * Cfg::W_BYTES);
+      const uint64_t bdesc = make_sw128_kmajor_desc(sbase + Cfg::OFF_X + s * Cfg::X_BYTES);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_ss(tmem_base, adesc + 2 * k, bdesc + 2 * k, idesc, (kb != kb0) || (k != 0));
+        umma_commit(bar_empty(s));
+      }
+      __syncwarp();
+      if (++s == STAGES) { s = 0; ph ^= 1; }
+    }
+    if (ok && elect_one()) umma_commit(bar_acc);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ accumulator -> own shared memory, [token][channel]
+    const int q = warp & 3;
+    if (mbar_wait_warp(bar_acc, 0, ctl, 2, 2 * STAGES, kb0)) {
+      tc_fence_after();
+      float* part = reinterpret_cast<float*>(smem);  // every operand has been read
+      const int ch = q * 32 + lane;
+      constexpr int HALVES = EW / 4;  // a quarter's two warps share the tokens
+      const int half = (warp - 2) >> 2;
+#pragma unroll
+      for (int hh = 0; hh < NT / 16 / HALVES; ++hh) {
+        const int h = hh * HALVES + half;
+        if (h * 16 >= tokens) break;
+        uint32_t v[16];
+        tmem_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + h * 16, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(h * 16 + j) * 128 + ch] = __uint_as_float(v[j]);
+      }
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  const int my_abort = ctl->abort;
+  if (S > 1) cluster_sync_all();
+  if (warp >= 2 && !my_abort) {
+    // ------------------------------------------------------------ this rank's tokens
+    const uint32_t part = sbase + lane * 16u;
+    if (S == 1) split_finish<1, EW>(p, part, m0, n0 + lane * 4, first, last, bias, res);
+    else if (S == 2) split_finish<2, EW>(p, part, m0, n0 + lane * 4, first, last, bias, res);
+    else if (S == 4) split_finish<4, EW>(p, part, m0, n0 + lane * 4, first, last, bias, res);
+    else split_finish<8, EW>(p, part, m0, n0 + lane * 4, first, last, bias, res);
+  }
+  // ------------------------------------------------------------ teardown
+  if (my_abort) {  // copies still in flight must land before the shared memory is given up
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  __syncthreads();
+  if (S > 1) cluster_sync_all();  // nobody leaves while a neighbour may still read its part
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace rl

@@ -26,7 +26,7 @@
 //   empty[s]    local        MMAs that read slot s are done            MMA commit (multicast) -> producers,
 //                                                                      and -> transform warps (A slot reuse)
 //   tfull[a]    local        accumulator a complete                    MMA commit (multicast) -> epilogues
-//   tempty[a]   rank 0 only  both epilogues drained accumulator a (8 arrivals) -> MMA warp
+//   tempty[a]   rank 0 only  both epilogues drained accumulator a (an arrival per epilogue warp) -> MMA warp
 //   rsfull[a]   local        row sums of squares written               transform -> own epilogue
 //   rsfree[a]   local        row sums consumed                         epilogue -> own transform warps
 #pragma once
@@ -72,7 +72,8 @@ struct PairCfg {
   static constexpr bool XFORM = (AMODE_ == A_TS_FOLD) || !PRESTATS_;
   static_assert(XFORM ? (TG_ > 0) : (TG_ == 0), "transform groups exactly where there is transform work");
   static_assert(!FP8_ || (!XFORM && !SWIGLU_ && BN_ == 256), "FP8: operands straight from shared memory");
-  static constexpr int THREADS = 64 + 128 * TG + 128;
+  static constexpr int EPI_WARPS = EPI_ ? 8 : 4;
+  static constexpr int THREADS = 64 + 128 * TG + 32 * EPI_WARPS;
   static constexpr int A_BYTES = 128 * 64 * 2;
   static constexpr int B_BYTES = (BN / 2) * 64 * 2;  // this CTA's half of the W tile
   static constexpr int G_BYTES = 128;
@@ -83,7 +84,7 @@ struct PairCfg {
   static constexpr int OFF_G = OFF_EPI + 2 * EPI_BYTES;
   static constexpr int OFF_RS = OFF_G + (AMODE_ == A_TS_FOLD ? STAGES * G_BYTES : 0);
   static constexpr int OFF_WS = OFF_RS + (PRESTATS_ ? 0 : TG * NACC * 128 * 4);  // FP8: [2][256] w_scale of the tiles being drained
-  static constexpr int OFF_BAR = OFF_WS + (FP8_ ? 2 * 256 * 4 : 0);
+  static constexpr int OFF_BAR = OFF_WS + (FP8_ ? 2 * 256 * 4 : 0) + (EPI_ ? 2 * BN_ * 2 : 0);  // (EPI: [2][BN] bias)
   static constexpr int NUM_BARS = 3 * STAGES + 4 * NACC;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int SMEM_BYTES = OFF_MISC + 64;  // no alignment slack: the kernel checks the base instead
@@ -131,6 +132,259 @@ __device__ __forceinline__ bool pair_item(const PrefillParams& p, int pair, int 
   w.kb0 = (int)(((long long)w.slice * KB) / S);
   w.kb1 = (int)(((long long)(w.slice + 1) * KB) / S);
   return true;
+}
+
+// Epilogue of the linear layer's configurations (PairCfg::EPI): y = act(acc + bias) + residual, rounded once.
+//
+// Eight warps in two groups of four: group g takes the 64-column chunks c = g, g + 2, .. of this CTA's 128 rows, each of its
+// warps 32 of them.  A thread owns one accumulator row, but the residual is loaded along the rows - a warp's 32 rows of a
+// chunk, one chunk ahead - and changes hands in the warp's 4 KB of the staging tiles, where the result takes its place and
+// leaves by a TMA store of the warp's own: no warp waits for another.  (Four warps and stores per group cost a third of the
+// layer on 4096 x 14336 x 4096; plain stores along the rows instead of TMA's cost 10-20 % more than these.)
+template <class Cfg>
+__device__ __forceinline__ void pair_linear_epilogue(const CUtensorMap* tm_y, const PrefillParams& p, uint8_t* smem,
+                                                     uint32_t sbase, uint32_t bar_tfull0, uint32_t lead_tempty0,
+                                                     uint32_t bar_tail, volatile int* epi_go, CtaCtl* ctl, uint32_t tmem_base,
+                                                     int rank, int pair, int n_pairs, int total_tiles, int KB) {
+  constexpr int BN = Cfg::BN, STAGES = Cfg::STAGES;
+  constexpr bool WIDE = Cfg::WIDE;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = (warp - 2) >> 2, q = warp & 3;
+  const int row = q * 32 + lane;
+  uint8_t* region = smem + Cfg::OFF_EPI + g * Cfg::EPI_BYTES + q * 4096;  // 32 rows x 128 bytes, swizzled
+  uint8_t* my_row = region + lane * 128;
+  const uint32_t swz = (uint32_t)(lane & 7);
+  unsigned short* bias_s = reinterpret_cast<unsigned short*>(smem + Cfg::OFF_WS);  // [2][BN] of the tiles being drained
+  const uint64_t pol_y = l2_policy_evict_first();
+  const bool has_res = p.residual != nullptr, res_vec = p.res_vec != 0;
+
+  // The residual of this warp's 32 rows, 64 columns from n0.  Rows on 16-byte boundaries: 16 bytes per lane, four rows at a
+  // time.  Otherwise two columns (lane, lane + 32) per lane and row.
+  uint32_t rr[32];
+  auto load_res = [&](int mt, int n0) {
+    const int m0 = mt * 256 + rank * 128 + q * 32;
+    if (res_vec) {
+      const int n = n0 + (lane & 7) * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int m = m0 + i * 4 + (lane >> 3);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (m < p.M && n < p.N) {
+          const __nv_bfloat16* src = p.residual + (size_t)m * p.ld_res + n;
+          if (n + 8 <= p.N) {
+            v = *reinterpret_cast<const uint4*>(src);
+          } else {
+            const uint2 lo = load4_bf16(src, n, p.N, false), hi = load4_bf16(src + 4, n + 4, p.N, false);
+            v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          }
+        }
+        rr[4 * i] = v.x; rr[4 * i + 1] = v.y; rr[4 * i + 2] = v.z; rr[4 * i + 3] = v.w;
+      }
+    } else {
+      const int n = n0 + lane;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const unsigned short* src = reinterpret_cast<const unsigned short*>(p.residual) + (size_t)(m0 + i) * p.ld_res + n;
+        const uint32_t lo = (m0 + i < p.M && n < p.N) ? src[0] : 0u, hi = (m0 + i < p.M && n + 32 < p.N) ? src[32] : 0u;
+        rr[i] = lo | (hi << 16);
+      }
+    }
+  };
+  // before a chunk is finished: the region is free again, and holds the residual
+  auto open_chunk = [&]() {
+    if (lane == 0) tma_store_wait_read<0>();
+    __syncwarp();
+    if (!has_res) return;
+    if (res_vec) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3);
+        *reinterpret_cast<uint4*>(region + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) =
+            make_uint4(rr[4 * i], rr[4 * i + 1], rr[4 * i + 2], rr[4 * i + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int at = (lane & 7) * 2;
+        *reinterpret_cast<unsigned short*>(region + i * 128 + (((lane >> 3) ^ (i & 7)) << 4) + at) = (unsigned short)rr[i];
+        *reinterpret_cast<unsigned short*>(region + i * 128 + (((4 + (lane >> 3)) ^ (i & 7)) << 4) + at) =
+            (unsigned short)(rr[i] >> 16);
+      }
+    }
+    __syncwarp();
+  };
+  // 16 columns of this thread's row (the qq-th of a chunk whose bias starts at `bias`), result into the region
+  auto finish16 = [&](uint64_t (&z)[8], const unsigned short* bias, int qq) {
+    uint4* at0 = reinterpret_cast<uint4*>(my_row + (((uint32_t)(2 * qq) ^ swz) << 4));
+    uint4* at1 = reinterpret_cast<uint4*>(my_row + (((uint32_t)(2 * qq + 1) ^ swz) << 4));
+    const uint4 b0 = *reinterpret_cast<const uint4*>(bias + qq * 16), b1 = *reinterpret_cast<const uint4*>(bias + qq * 16 + 8);
+    uint4 r0 = make_uint4(0u, 0u, 0u, 0u), r1 = r0;
+    if (has_res) { r0 = *at0; r1 = *at1; }
+    const uint32_t bw[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+    const uint32_t rw[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+    uint32_t o[8];
+    linear_epilogue(z, bw, rw, p.act, o);
+    *at0 = make_uint4(o[0], o[1], o[2], o[3]);
+    *at1 = make_uint4(o[4], o[5], o[6], o[7]);
+  };
+  auto close_chunk = [&](int mt, int n0) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    const int m = mt * 256 + rank * 128 + q * 32;
+    if (lane == 0) {
+      if (n0 < p.N && m < p.M) tma_store_2d_hint(tm_y, smem_u32(region), n0, m, pol_y);
+      tma_store_commit();
+    }
+  };
+
+  bool ok = true;
+  PairItem w;
+  for (int it = 0; ok && pair_item<true>(p, pair, n_pairs, total_tiles, KB, it, w); ++it) {
+    int mt, nt;
+    prefill_tile_coords(w.t, p, mt, nt);
+    const int acc = WIDE ? 0 : (it & 1);
+    const uint32_t aph = WIDE ? (it & 1) : ((it >> 1) & 1);
+    // a k-slice finishes columns c_lo .. c_lo + nch - 1 of the tile's chunks, a whole tile all of them
+    const int S = w.slice >= 0 ? p.tail_split : 1, slice = w.slice >= 0 ? w.slice : 0;
+    const int c_lo = (slice * (BN / 64)) / S, nch = ((slice + 1) * (BN / 64)) / S - c_lo;
+    // bias and first residual are on their way while the accumulator fills (the buffer of the tile before last is free:
+    // every thread has passed the barriers of the last one)
+    unsigned short* bias = bias_s + (it & 1) * BN;
+#pragma unroll
+    for (int j = 0; j < BN; j += 256) {
+      const int at = j + (int)threadIdx.x - 64, n = nt * BN + at;
+      bias[at] = (p.bias != nullptr && n < p.N) ? reinterpret_cast<const unsigned short*>(p.bias)[n] : (unsigned short)0;
+    }
+    if (has_res && g < nch) load_res(mt, nt * BN + (c_lo + g) * 64);
+    mbar_wait_long(bar_tfull0 + 8u * acc, aph, ctl, 3, 3 * STAGES + acc, it);
+    // named barriers have no time limit: one thread decides for both groups whether to go on
+    named_bar_sync(1, 256);
+    if (threadIdx.x == 64) epi_go[0] = ctl->abort ? 0 : 1;
+    named_bar_sync(1, 256);
+    ok = (epi_go[0] != 0);
+    if (!ok) break;
+    tc_fence_after();
+    const uint32_t trow = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN;
+    if (w.slice < 0) {
+#pragma unroll 1
+      for (int c = g; c < BN / 64; c += 2) {
+        uint32_t v[2][16];
+        tmem_ld16(trow + c * 64, v[0]);
+        open_chunk();
+        if (has_res && c + 2 < BN / 64) load_res(mt, nt * BN + (c + 2) * 64);
+#pragma unroll
+        for (int qq = 0; qq < 4; ++qq) {
+          tmem_wait_ld();
+          if (qq < 3) {
+            tmem_ld16(trow + c * 64 + (qq + 1) * 16, v[(qq + 1) & 1]);
+          } else if (c >= BN / 64 - 2 || (WIDE && (c == 2 || c == 3))) {
+            // this warp has the last of the accumulator (WIDE: of this half of it) in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(lead_tempty0 + 8u * (WIDE ? (c > 3 ? 1 : 0) : acc));
+          }
+          uint64_t z[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) z[j] = pack2(__uint_as_float(v[qq & 1][2 * j]), __uint_as_float(v[qq & 1][2 * j + 1]));
+          finish16(z, bias + c * 64, qq);
+        }
+        close_chunk(mt, nt * BN + c * 64);
+      }
+      continue;
+    }
+    // ---- one k-slice of a tail tile (always this pair's last item): the exchange of prefill_pair_kernel's own epilogue,
+    // with the columns of both the partial blocks and the finished share dealt to the two groups
+    const int tl = w.t - (total_tiles - p.tail_tiles);
+    unsigned* cnt = p.tail_counters + 2 * (tl * 2 + rank);  // [0] partials written, [1] waits passed
+    constexpr int SLOT_F4 = 128 * BN / 4;
+    constexpr uint32_t PART_BYTES = 64 * 128 * 4;
+    constexpr uint32_t PART_BUFS = (BN == 512) ? 6 : 4;
+    static_assert(PART_BUFS * PART_BYTES <= (uint32_t)Cfg::OFF_EPI, "partial buffers fit in the operand ring");
+    float4* slot0 = reinterpret_cast<float4*>(p.tail_partials) + (size_t)(tl * S * 2 + rank) * SLOT_F4;
+    float4* mine = slot0 + (size_t)slice * 2 * SLOT_F4;
+#pragma unroll 1
+    for (int c = g; c < BN / 64; c += 2) {
+      if (c >= c_lo && c < c_lo + nch) continue;  // these stay in tensor memory
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[32];
+        tmem_ld32(trow + c * 64 + h * 32, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          mine[(c * 16 + h * 8 + j) * 128 + row] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
+                                                               __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+      }
+    }
+    __threadfence();
+    named_bar_sync(1, 256);
+    if (threadIdx.x == 64) {
+      atomicAdd(cnt, 1u);
+      const bool good = global_count_wait(cnt, (unsigned)S, ctl, 3, 100 + tl, it);
+      if (good) {
+        __threadfence();
+        asm volatile("fence.proxy.async.global;" ::: "memory");  // the bulk copies below read what others wrote
+        mbar_expect_tx(bar_tail, (uint32_t)((S - 1) * nch) * PART_BYTES);
+        int b = 0;
+        for (int sl = 0; sl < S; ++sl) {
+          if (sl == slice) continue;
+          for (int c = 0; c < nch; ++c, ++b)
+            bulk_load_1d(sbase + (uint32_t)b * PART_BYTES, slot0 + (size_t)sl * 2 * SLOT_F4 + (size_t)(c_lo + c) * 16 * 128,
+                         PART_BYTES, bar_tail);
+        }
+        // the last of the S to get here puts the pair of counters back to zero for the next launch
+        if (atomicAdd(cnt + 1, 1u) == (unsigned)(S - 1)) {
+          cnt[0] = 0u;
+          cnt[1] = 0u;
+        }
+      }
+      epi_go[0] = good ? 1 : 0;
+    }
+    named_bar_sync(1, 256);
+    ok = (epi_go[0] != 0);
+    if (!ok) break;
+    mbar_wait(bar_tail, 0u, ctl, 3, 200 + tl, it);
+    named_bar_sync(1, 256);
+    if (threadIdx.x == 64) epi_go[0] = ctl->abort ? 0 : 1;
+    named_bar_sync(1, 256);
+    ok = (epi_go[0] != 0);
+    if (!ok) break;
+#pragma unroll 1
+    for (int c = g; c < nch; c += 2) {
+      open_chunk();
+      if (has_res && c + 2 < nch) load_res(mt, nt * BN + (c_lo + c + 2) * 64);
+#pragma unroll 1
+      for (int qq = 0; qq < 4; ++qq) {
+        uint32_t own[16];
+        tmem_ld16(trow + (c_lo + c) * 64 + qq * 16, own);
+        uint64_t z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = 0ull;
+        tmem_wait_ld();
+        int b = 0;
+#pragma unroll 1
+        for (int sl = 0; sl < S; ++sl) {  // slice order, this CTA's own slice in its place
+          if (sl == slice) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              z[j] = add2(z[j], pack2(__uint_as_float(own[2 * j]), __uint_as_float(own[2 * j + 1])));
+          } else {
+            const float4* ps = reinterpret_cast<const float4*>(smem + (size_t)(b * nch + c) * PART_BYTES) + (qq * 4) * 128 + row;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 d4 = ps[j * 128];
+              z[2 * j] = add2(z[2 * j], pack2(d4.x, d4.y));
+              z[2 * j + 1] = add2(z[2 * j + 1], pack2(d4.z, d4.w));
+            }
+            ++b;
+          }
+        }
+        finish16(z, bias + (c_lo + c) * 64, qq);
+      }
+      close_chunk(mt, nt * BN + (c_lo + c) * 64);
+    }
+  }
+  if (lane == 0) tma_store_wait_all<0>();
 }
 
 template <class Cfg>
@@ -188,7 +442,7 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
     }
     for (int a = 0; a < NACC; ++a) {
       mbar_init(bar_tfull(a), 1);
-      mbar_init(bar_tempty(a), 8);
+      mbar_init(bar_tempty(a), 2 * Cfg::EPI_WARPS);
       mbar_init(bar_rsfull(a), XFORM ? 4 * TG : 1);
       mbar_init(bar_rsfree(a), 4);
     }
@@ -214,6 +468,9 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
   cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // the linear layer is launched as a programmatic dependent of whatever runs in front of it: nothing in global memory is
+  // touched before that is complete
+  if (EPI) grid_dependency_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs, own halves)
@@ -436,6 +693,9 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
         if (lane == 0) mbar_arrive(bar_rsfull(acc));
       }
     }
+  } else if constexpr (EPI) {
+    pair_linear_epilogue<Cfg>(&tm_y, p, smem, sbase, bar_tfull(0), mapa_shared(bar_tempty(0), 0), bar_tail, epi_go, ctl,
+                              tmem_base, (int)rank, pair, n_pairs, total_tiles, KB);
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs, own 128 rows)
     const int q = warp & 3;
@@ -500,24 +760,6 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             o[j] = pack_bf16x2(__uint_as_float(v[2 * j]) * r, __uint_as_float(v[2 * j + 1]) * r);
-        }
-      };
-      // EPI: 16 columns of the bias, and of this thread's row of the residual, from column n of y
-      [[maybe_unused]] auto load_bias16 = [&](int n, uint32_t (&w)[8]) {
-        if (p.bias == nullptr) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = 0u;
-        } else {
-          load16_bf16(p.bias + n, n, p.N, true, w);
-        }
-      };
-      [[maybe_unused]] auto load_res16 = [&](int n, uint32_t (&w)[8]) {
-        const int m = mt * 256 + (int)rank * 128 + row;
-        if (p.residual == nullptr || m >= p.M) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = 0u;
-        } else {
-          load16_bf16(p.residual + (size_t)m * p.ld_res + n, n, p.N, p.res_vec != 0, w);
         }
       };
       // write 64 columns (two 16-word halves) of this thread's row into a swizzled staging tile
@@ -637,22 +879,15 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
                   ++b;
                 }
               }
-              if constexpr (EPI) {
-                uint32_t rw[8], bw[8];
-                load_res16(nt * BN + (c_lo + c) * 64 + qq * 16, rw);
-                load_bias16(nt * BN + (c_lo + c) * 64 + qq * 16, bw);
-                epilogue16(a, bw, rw, p.act, &o[qq >> 1][(qq & 1) * 8]);
-              } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  float s0 = r, s1 = r;
-                  if constexpr (FP8) {
-                    const float2 ws2 = *reinterpret_cast<const float2*>(wc_tile + (c_lo + c) * 64 + qq * 16 + 2 * j);
-                    s0 *= ws2.x;
-                    s1 *= ws2.y;
-                  }
-                  o[qq >> 1][(qq & 1) * 8 + j] = pack_bf16x2(a[2 * j] * s0, a[2 * j + 1] * s1);
+              for (int j = 0; j < 8; ++j) {
+                float s0 = r, s1 = r;
+                if constexpr (FP8) {
+                  const float2 ws2 = *reinterpret_cast<const float2*>(wc_tile + (c_lo + c) * 64 + qq * 16 + 2 * j);
+                  s0 *= ws2.x;
+                  s1 *= ws2.y;
                 }
+                o[qq >> 1][(qq & 1) * 8 + j] = pack_bf16x2(a[2 * j] * s0, a[2 * j + 1] * s1);
               }
             }
             sts64(stage, o[0], o[1]);
@@ -813,22 +1048,8 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
             if (lane == 0) mbar_arrive_cluster(lead_tempty0 + 8u * (WIDE ? (c > 3 ? 1 : 0) : acc));
           }
           uint32_t lo[16], hi[16];
-          if constexpr (EPI) {
-#pragma unroll
-            for (int qq = 0; qq < 4; ++qq) {
-              const uint32_t(&v)[32] = (qq < 2) ? v0 : v1;
-              uint32_t rw[8], bw[8];
-              load_res16(nt * BN + c * 64 + qq * 16, rw);
-              load_bias16(nt * BN + c * 64 + qq * 16, bw);
-              float z[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) z[j] = __uint_as_float(v[(qq & 1) * 16 + j]);
-              epilogue16(z, bw, rw, p.act, (qq < 2 ? lo : hi) + (qq & 1) * 8);
-            }
-          } else {
-            cvt32(v0, lo, c * 64);
-            cvt32(v1, hi, c * 64 + 32);
-          }
+          cvt32(v0, lo, c * 64);
+          cvt32(v1, hi, c * 64 + 32);
           sts64(stage, lo, hi);
           fence_proxy_async_smem();
           named_bar_sync(2, 128);

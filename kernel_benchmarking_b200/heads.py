@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _index_devices, _raw_stream
+from .ops import _status_devices, _raw_stream
 
 
 # The checks sit on the path of every decode step, whose kernels run for a few microseconds: each call makes them as one
@@ -116,7 +116,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: Optional[torch.Tenso
                k_t, k_h, qo_t, qo_h, ko_t, ko_h, eps, interleaved)
     if rc:
         _lib.check(rc, "rl_qk_norm_rope_bf16")
-    _index_devices.add(dev)
+    _status_devices.add(dev)
     return qo, ko
 
 
@@ -182,7 +182,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_code
                c_page, c_off, c_head, s_page, s_off, s_head)
     if rc:
         _lib.check(rc, "rl_kv_cache_write_e4m3")
-    _index_devices.add(dev)
+    _status_devices.add(dev)
 
 
 def kv_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
@@ -227,5 +227,5 @@ def kv_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.T
                H, D, pages, page_size, c_page, c_off, c_head, s_page, s_off, s_head, ko_t, ko_h, vo_t, vo_h)
     if rc:
         _lib.check(rc, "rl_kv_cache_read_e4m3")
-    _index_devices.add(dev)
+    _status_devices.add(dev)
     return ko, vo

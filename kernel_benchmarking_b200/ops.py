@@ -18,7 +18,7 @@ from . import _lib
 
 _workspaces: dict = {}
 _own_workspaces: dict = {}   # id -> weak reference: what linear_workspace handed out
-_index_devices: set = set()  # devices on which an operator that takes positions, slots or pages has run
+_status_devices: set = set()  # devices on which a kernel without a workspace has run
 _CLEAN_BYTES = 256 + 65536   # status block and tile counters: the part of a workspace that starts from zero
 
 
@@ -246,8 +246,8 @@ def lora_linear(a: torch.Tensor, b: torch.Tensor, lA: torch.Tensor, lB: torch.Te
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_workspace_bytes(M: int, N: int) -> int:
-    return _lib.load().rl_linear_workspace_bytes(M, N)
+def _linear_workspace_bytes(M: int, N: int, K: int) -> int:
+    return _lib.load().rl_linear_workspace_bytes(M, N, K)
 
 
 def _matrix_ok(t: torch.Tensor, dev: int) -> bool:
@@ -255,13 +255,14 @@ def _matrix_ok(t: torch.Tensor, dev: int) -> bool:
             and t.stride(1) == 1)
 
 
-def linear_workspace(M: int, N: int, device: Optional[torch.device] = None) -> torch.Tensor:
-    """Scratch for `linear(..., workspace=...)` calls of up to M tokens and N channels (M <= 64 and M > 64 lay theirs out
-    differently: ask with the M of the call).  For calls captured into CUDA graphs: a workspace of one's own is zeroed
-    here, once, and not on every replay.  Calls that share it must not overlap on the device."""
-    ws = torch.zeros(_lib.load().rl_linear_workspace_bytes(M, N), dtype=torch.uint8, device=device or "cuda")
+def linear_workspace(M: int, N: int, K: int, device: Optional[torch.device] = None) -> torch.Tensor:
+    """Scratch for `linear(..., workspace=...)` calls of M tokens, N channels and K (empty where the call needs none).
+    For calls captured into CUDA graphs: a workspace of one's own is zeroed here, once, and not on every replay.  Calls
+    that share it must not overlap on the device."""
+    ws = torch.zeros(_linear_workspace_bytes(M, N, K), dtype=torch.uint8, device=device or "cuda")
     key = id(ws)
-    _own_workspaces[key] = weakref.ref(ws, lambda _: _own_workspaces.pop(key, None))
+    if ws.numel():   # check_status reads its status block
+        _own_workspaces[key] = weakref.ref(ws, lambda _: _own_workspaces.pop(key, None))
     return ws
 
 
@@ -272,12 +273,12 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
     the one rounding of the result.  The projection behind an attention or an MLP, added to the residual stream.
 
     `activation`: None, "relu", "gelu" (erf), "gelu_tanh" or "silu".  `residual` may be `out` itself (an update in
-    place); `out` may share no other memory with the inputs.  Up to 64 tokens run the weight-streaming kernel, more the
-    tensor-core tiles.  `variant="auto_whole"` on streams that run concurrently (see `rmsnorm_linear`).
+    place), or one row expanded to all tokens; `out` may share no other memory with the inputs.
 
-    Scratch: one workspace per device and stream, as for the other operators.  A call that is being captured into a CUDA
-    graph takes one of its own from the graph's memory and clears it on every replay, so graphs share none; a
-    `linear_workspace` passed in saves that step."""
+    Few tokens or few tiles need no scratch.  The others use one workspace per device and stream, as the other operators
+    do, and `variant="auto_whole"` belongs on streams that run concurrently (see `rmsnorm_linear`).  A call that is being
+    captured into a CUDA graph takes a workspace of its own from the graph's memory and clears it on every replay, so
+    graphs share none; a `linear_workspace` passed in saves that step."""
     # one plain condition on the path of every decode step; what is wrong is looked for only when it fails
     dev = x.get_device() if isinstance(x, torch.Tensor) and x.is_cuda else None
     if dev is None or not (_matrix_ok(x, dev) and _matrix_ok(W, dev) and (residual is None or _matrix_ok(residual, dev))):
@@ -309,7 +310,7 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
         _check_out(out, M, N, x)
     if M == 0 or N == 0:
         return out
-    nbytes = _linear_workspace_bytes(M, N)
+    nbytes = _linear_workspace_bytes(M, N, K)
     if workspace is not None and not (isinstance(workspace, torch.Tensor) and workspace.get_device() == dev
                                       and workspace.dtype is torch.uint8 and workspace.is_contiguous()
                                       and workspace.numel() >= nbytes):
@@ -327,16 +328,21 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
 def _launch_linear(dev, x, W, bias, residual, out, M, N, K, act, ws, nbytes, variant) -> int:
     lib = _lib.load()
     stream = _raw_stream(dev)
-    if ws is None:
+    if nbytes == 0:
+        ws_ptr = ws_bytes = 0
+        _status_devices.add(dev)
+    elif ws is None:
         if torch.cuda.is_current_stream_capturing():
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
             _lib.check(lib.rl_workspace_init(ws.data_ptr(), _CLEAN_BYTES, stream), "rl_workspace_init")
         else:
             ws = _workspace(x.device, nbytes, stream)
+    if nbytes:
+        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
     return lib.rl_linear_bf16(x.data_ptr(), W.data_ptr(), None if bias is None else bias.data_ptr(),
                               None if residual is None else residual.data_ptr(), out.data_ptr(), M, N, K, x.stride(0),
-                              W.stride(0), 0 if residual is None else residual.stride(0), out.stride(0), act, ws.data_ptr(),
-                              ws.numel(), _lib.VARIANTS[variant], stream)
+                              W.stride(0), 0 if residual is None else residual.stride(0), out.stride(0), act, ws_ptr, ws_bytes,
+                              _lib.VARIANTS[variant], stream)
 
 
 def quantize_rows_e4m3(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-6):
@@ -396,14 +402,16 @@ def check_status(device: Optional[torch.device] = None) -> None:
                 torch.cuda.synchronize()
                 if first_error is None:
                     first_error = f"rmsnorm_linear: {_lib.error_string(rc)}; detail={list(detail)}"
-    for dev in list(_index_devices):
+    for dev in list(_status_devices):
         if device is not None and torch.device(device).index not in (None, dev):
             continue
         detail = (ctypes.c_int * 4)()
         with torch.cuda.device(dev):
             torch.cuda.synchronize()
-            rc = lib.rl_take_index_status(detail)
-        if rc != _lib.RL_OK and first_error is None:
+            rc = lib.rl_take_device_status(detail)
+        if rc != _lib.RL_OK and rc != _lib.RL_ERR_BAD_INDEX and first_error is None:
+            first_error = f"linear: {_lib.error_string(rc)}; detail={list(detail)}"
+        elif rc == _lib.RL_ERR_BAD_INDEX and first_error is None:
             kind = {1: "position", 2: "slot", 3: "page"}.get(detail[0], "index")
             first_error = (f"{_lib.error_string(rc)}: {kind} {(detail[2] & 0xffffffff) | (detail[3] << 32)}, "
                            f"row {detail[1]} of the call, cuda:{dev}")

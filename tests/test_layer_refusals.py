@@ -20,6 +20,9 @@ def lib():
 A = [0x10000000 * (i + 1) for i in range(10)]
 
 
+FAR = {k: 0x100000000 * (i + 1) for i, k in enumerate(("x", "W", "bias", "res", "y"))}   # for matrices of many megabytes
+
+
 def passed(rc):
     """The argument checks let the call through: on a machine without a GPU it then fails in the CUDA runtime."""
     return rc <= _lib.RL_ERR_CUDA or rc in (_lib.RL_OK, _lib.RL_ERR_UNSUPPORTED_ARCH)
@@ -41,8 +44,8 @@ def call_linear(lib, x=A[0], W=A[1], bias=A[2], res=A[3], y=A[4], M=128, N=128, 
     (ALIGN, dict(ldy=130)), (ALIGN, dict(y=A[4] + 2)), (ALIGN, dict(res=A[3] + 1)),
     (_lib.RL_ERR_BAD_ACTIVATION, dict(act=5)), (_lib.RL_ERR_BAD_ACTIVATION, dict(act=-1)),
     (_lib.RL_ERR_BAD_VARIANT, dict(variant=20)),
-    (_lib.RL_ERR_WORKSPACE, dict(ws=None)), (_lib.RL_ERR_WORKSPACE, dict(ws_bytes=256)),
-    (_lib.RL_ERR_WORKSPACE, dict(M=16, ws_bytes=256)),
+    (_lib.RL_ERR_WORKSPACE, dict(M=4096, N=4096, K=4096, ws=None, ldx=4096, ldw=4096, ldr=4096, ldy=4096, **FAR)),
+    (_lib.RL_ERR_WORKSPACE, dict(M=4096, N=4096, K=4096, ws_bytes=256, ldx=4096, ldw=4096, ldr=4096, ldy=4096, **FAR)),
     (OVERLAP, dict(y=A[0])), (OVERLAP, dict(y=A[1] + 1024)), (OVERLAP, dict(bias=A[4] + 128 * 128 * 2 - 16)),
     (OVERLAP, dict(res=A[4] + 256)),                 # the residual one row ahead of y
     (OVERLAP, dict(res=A[4], ldr=136)),              # the same start, other rows
@@ -59,9 +62,17 @@ def test_linear_accepts(lib):
     assert passed(call_linear(lib, res=A[3] + 2, ldr=129))                     # rows of the residual need no alignment
     assert passed(call_linear(lib, M=16, ldy=129, y=A[4] + 2))                 # nor those of y for small M
     assert passed(call_linear(lib, bias=None, res=None, ldr=0))
-    assert lib.rl_linear_workspace_bytes(0, 8) == 256
-    assert lib.rl_linear_workspace_bytes(16, 4096) == lib.rl_workspace_bytes(16, 4096, 4096, 0)
-    assert lib.rl_linear_workspace_bytes(8192, 28672) < lib.rl_workspace_bytes(8192, 28672, 8192, 0)  # no folded copy of x
+    assert passed(call_linear(lib, ws=None, ws_bytes=0))                       # few tiles need no workspace
+
+
+def test_linear_workspace_bytes(lib):
+    f = lib.rl_linear_workspace_bytes
+    assert f(0, 8, 8) == f(8, 0, 8) == f(8, 8, 0) == 0
+    for M in (1, 16, 64):
+        assert f(M, 4096, 4096) == f(M, 57344, 8192) == 0
+    assert f(333, 1000, 1144) == f(128, 4096, 4096) == f(512, 4096, 4096) == 0
+    assert f(8192, 4096, 4096) == lib.rl_workspace_bytes(8192, 4096, 4096, 0)
+    assert 0 < f(8192, 28672, 8192) < lib.rl_workspace_bytes(8192, 28672, 8192, 0)   # no folded copy of x
 
 
 def call_qk(lib, q=A[0], k=A[1], gq=A[2], gk=A[3], table=A[4], pos=A[5], p64=1, qo=A[6], ko=A[7], T=64, Hq=8, Hk=2, D=64, rot=64,
