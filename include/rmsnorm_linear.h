@@ -247,10 +247,17 @@ int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* r
  *   ld_table of 4; pointers 16-byte aligned.
  *   A position outside the table: that token's rows are not written, and rl_take_device_status reports it.
  * No workspace.  No reference counterpart. */
-int rl_qk_norm_rope_bf16(const void* q, const void* k, const void* q_gamma, const void* k_gamma, const float* table,
-                         const void* positions, int positions_i64, void* q_out, void* k_out, int T, int Hq, int Hk, int D,
-                         int rot, int n_positions, int64_t ld_table, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h,
-                         int64_t qo_t, int64_t qo_h, int64_t ko_t, int64_t ko_h, float eps, int interleaved, void* stream);
+typedef struct {
+  const void *q, *k, *q_gamma, *k_gamma;
+  const float* table;
+  const void* positions;
+  void *q_out, *k_out;
+  int64_t T, Hq, Hk, D, rot, n_positions, ld_table;
+  int64_t q_t, q_h, k_t, k_h, qo_t, qo_h, ko_t, ko_h;
+  int64_t positions_i64, interleaved;
+  double eps;
+} rl_qk_norm_rope_args;
+int rl_qk_norm_rope_bf16(const rl_qk_norm_rope_args* args, void* stream);
 
 /* Keys and values into a paged e4m3 cache, one fp32 scale per (token, head), the scale found as the row is written:
  *   a = max(max_d |x_d|, 2^-100), scale = a / 448, code_d = e4m3(448 x_d / a) (the exact quotient, ties to even).
@@ -262,10 +269,19 @@ int rl_qk_norm_rope_bf16(const void* q, const void* k, const void* q_gamma, cons
  *   must differ: where two tokens name one slot, its codes and scale may come from either.
  *   D a multiple of 8, at most 256; strides of k, v and the codes multiples of 8; k, v 16-byte, codes 8-byte aligned.
  * No workspace.  No reference counterpart. */
-int rl_kv_cache_write_e4m3(const void* k, const void* v, const void* slots, int slots_i64, void* k_codes, float* k_scale,
-                           void* v_codes, float* v_scale, int T, int H, int D, int num_pages, int page_size, int64_t k_t,
-                           int64_t k_h, int64_t v_t, int64_t v_h, int64_t code_page, int64_t code_token, int64_t code_head,
-                           int64_t scale_page, int64_t scale_token, int64_t scale_head, void* stream);
+typedef struct {
+  void *k_codes, *v_codes;
+  float *k_scale, *v_scale;
+  int64_t num_pages, page_size, H, D;
+  int64_t code_page, code_token, code_head;     /* strides of the codes (bytes = elements) */
+  int64_t scale_page, scale_token, scale_head;  /* strides of the scales in elements */
+} rl_kv_cache_e4m3;
+typedef struct {
+  rl_kv_cache_e4m3 cache;
+  const void *k, *v, *slots;
+  int64_t T, k_t, k_h, v_t, v_h, slots_i64;
+} rl_kv_cache_write_args;
+int rl_kv_cache_write_e4m3(const rl_kv_cache_write_args* args, void* stream);
 
 /* The cache back as bf16(code * scale), the sequences packed one behind the other: row cu_seqlens[b] + i of k_out and
  * v_out [total, H, D] is token i of sequence b, which lies in page page_table[b, i / page_size].
@@ -274,11 +290,13 @@ int rl_kv_cache_write_e4m3(const void* k, const void* v, const void* slots, int 
  *   A page outside the cache, or a sequence longer than its table row: the row is left as it is and
  *   rl_take_device_status reports it.
  * Cache arguments and alignments as for rl_kv_cache_write_e4m3.  No workspace.  No reference counterpart. */
-int rl_kv_cache_read_e4m3(const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
-                          const int* page_table, const int* cu_seqlens, void* k_out, void* v_out, int total, int zero_tail,
-                          int B, int max_pages, int64_t ld_pages, int H, int D, int num_pages, int page_size, int64_t code_page,
-                          int64_t code_token, int64_t code_head, int64_t scale_page, int64_t scale_token, int64_t scale_head,
-                          int64_t ko_t, int64_t ko_h, int64_t vo_t, int64_t vo_h, void* stream);
+typedef struct {
+  rl_kv_cache_e4m3 cache;
+  const int *page_table, *cu_seqlens;
+  void *k_out, *v_out;
+  int64_t total, zero_tail, B, max_pages, ld_pages, ko_t, ko_h, vo_t, vo_h;
+} rl_kv_cache_read_args;
+int rl_kv_cache_read_e4m3(const rl_kv_cache_read_args* args, void* stream);
 
 /* What the kernels without a workspace recorded on the current device since this was last called (it clears the record;
  * call it outside the hot loop, with the streams synchronised): the first position, slot or page that a kernel of the

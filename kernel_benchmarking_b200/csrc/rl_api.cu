@@ -782,13 +782,13 @@ inline int pick_steps(int tokens, int groups, int sms) {
   return (int)std::max(1LL, std::min<long long>({n, groups, 16}));
 }
 template <class Params>
-int launch_rows(void (*kernel)(Params), const Params& p, cudaStream_t st) {
-  const long long blocks = ((long long)p.T * p.parts + 3) / 4;
+int launch_rows(void (*kernel)(Params), int warps, const Params& p, cudaStream_t st) {
+  const long long blocks = ((long long)p.T * p.parts + warps - 1) / warps;
   if (blocks > 0x7fffffffLL) return RL_ERR_BAD_SHAPE;
   // a programmatic dependent: the kernels touch no global memory before griddepcontrol.wait
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)blocks);
-  lc.blockDim = dim3(128);
+  lc.blockDim = dim3(32 * warps);
   lc.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -812,6 +812,11 @@ inline bool mult8(std::initializer_list<int64_t> v) {
     if (x & 7) return false;
   return true;
 }
+inline bool fit_int(std::initializer_list<int64_t> v) {
+  for (int64_t x : v)
+    if (x < -0x7fffffffLL || x > 0x7fffffffLL) return false;
+  return true;
+}
 inline bool nonneg(std::initializer_list<int64_t> v) {
   for (int64_t x : v)
     if (x < 0) return false;
@@ -819,14 +824,17 @@ inline bool nonneg(std::initializer_list<int64_t> v) {
 }
 
 // what the two cache entry points check about the cache itself
-int check_cache(const KvCache& c) {
-  if (!c.k_codes || !c.v_codes || !c.k_scale || !c.v_scale) return RL_ERR_NULL_POINTER;
-  if (c.num_pages < 0 || c.page_size <= 0 || c.H <= 0 || c.D <= 0 || c.D > 256 ||
-      !nonneg({c.c_page, c.c_off, c.c_head, c.s_page, c.s_off, c.s_head}))
+int check_cache(const rl_kv_cache_e4m3& a, KvCache* out) {
+  if (!a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale) return RL_ERR_NULL_POINTER;
+  if (!fit_int({a.num_pages, a.page_size, a.H, a.D}) || a.num_pages < 0 || a.page_size <= 0 || a.H <= 0 || a.D <= 0 || a.D > 256 ||
+      !nonneg({a.code_page, a.code_token, a.code_head, a.scale_page, a.scale_token, a.scale_head}))
     return RL_ERR_BAD_SHAPE;
+  const KvCache c{(uint8_t*)a.k_codes, (uint8_t*)a.v_codes, a.k_scale, a.v_scale, a.code_page, a.code_token, a.code_head,
+                  a.scale_page, a.scale_token, a.scale_head, (int)a.num_pages, (int)a.page_size, (int)a.H, (int)a.D};
   const uintptr_t codes = reinterpret_cast<uintptr_t>(c.k_codes) | reinterpret_cast<uintptr_t>(c.v_codes);
   const uintptr_t scales = reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale);
   if ((codes & 7) || (scales & 3) || !mult8({c.D, c.c_page, c.c_off, c.c_head})) return RL_ERR_ALIGNMENT;
+  *out = c;
   return RL_OK;
 }
 View code_view(const KvCache& c, const void* p) {
@@ -1214,11 +1222,14 @@ int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* r
   return launch_prefill_pair<PairLinear>(pa);
 }
 
-int rl_qk_norm_rope_bf16(const void* q, const void* k, const void* q_gamma, const void* k_gamma, const float* table,
-                         const void* positions, int positions_i64, void* q_out, void* k_out, int T, int Hq, int Hk, int D,
-                         int rot, int n_positions, int64_t ld_table, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h,
-                         int64_t qo_t, int64_t qo_h, int64_t ko_t, int64_t ko_h, float eps, int interleaved, void* stream) {
+int rl_qk_norm_rope_bf16(const rl_qk_norm_rope_args* args, void* stream) {
+  if (!args) return RL_ERR_NULL_POINTER;
+  const rl_qk_norm_rope_args& a = *args;
+  const auto [q, k, q_gamma, k_gamma, table, positions, q_out, k_out, T64, Hq64, Hk64, D64, rot64, n_positions64, ld_table, q_t, q_h,
+              k_t, k_h, qo_t, qo_h, ko_t, ko_h, positions_i64, interleaved, eps] = a;
   if (!q || !k || !table || !positions || !q_out || !k_out) return RL_ERR_NULL_POINTER;
+  if (!fit_int({T64, Hq64, Hk64, D64, rot64, n_positions64})) return RL_ERR_BAD_SHAPE;
+  const int T = (int)T64, Hq = (int)Hq64, Hk = (int)Hk64, D = (int)D64, rot = (int)rot64, n_positions = (int)n_positions64;
   if (T <= 0 || Hq <= 0 || Hk <= 0 || D <= 0 || D > 256 || rot <= 0 || rot > D || n_positions < 0 || ld_table < rot ||
       (long long)Hq + Hk > 65536 || !nonneg({q_t, q_h, k_t, k_h, qo_t, qo_h, ko_t, ko_h}))
     return RL_ERR_BAD_SHAPE;
@@ -1242,38 +1253,41 @@ int rl_qk_norm_rope_bf16(const void* q, const void* k, const void* q_gamma, cons
   p.q = reinterpret_cast<const __nv_bfloat16*>(q); p.k = reinterpret_cast<const __nv_bfloat16*>(k);
   p.q_gamma = reinterpret_cast<const __nv_bfloat16*>(q_gamma); p.k_gamma = reinterpret_cast<const __nv_bfloat16*>(k_gamma);
   p.q_out = reinterpret_cast<__nv_bfloat16*>(q_out); p.k_out = reinterpret_cast<__nv_bfloat16*>(k_out);
-  p.table = table; p.positions = positions; p.pos64 = positions_i64; p.n_pos = n_positions;
+  p.table = table; p.positions = positions; p.pos64 = positions_i64 != 0; p.n_pos = n_positions;
   p.T = T; p.Hq = Hq; p.Hk = Hk; p.D = D; p.rot = rot; p.ld_table = ld_table;
   p.q_t = q_t; p.q_h = q_h; p.k_t = k_t; p.k_h = k_h; p.qo_t = qo_t; p.qo_h = qo_h; p.ko_t = ko_t; p.ko_h = ko_h;
-  p.eps = eps;
+  p.eps = (float)eps;
   const int G = lanes_per_row(D), R = 32 / G;
-  const int q_groups = (Hq + R - 1) / R, k_groups = (Hk + R - 1) / R;
-  p.steps = pick_steps(T, q_groups + k_groups, di.sms);
-  p.q_parts = (q_groups + p.steps - 1) / p.steps;
-  p.parts = p.q_parts + (k_groups + p.steps - 1) / p.steps;
+  const int groups = (Hq + R - 1) / R + (Hk + R - 1) / R;
+  p.steps = pick_steps(T, groups, di.sms);
+  p.parts = (groups + p.steps - 1) / p.steps;
   cudaStream_t st = (cudaStream_t)stream;
   // (a head of one lane turns inside it: rot is 16 there, or the pairs are neighbours)
-#define RL_CALL(g) launch_rows(interleaved ? qk_rope_kernel<g, MATE_NEIGHBOUR> : rot == 16 * g ? qk_rope_kernel<g, MATE_OTHER_CHUNK> \
-                                                                                             : qk_rope_kernel<g, (g == 1 ? MATE_OTHER_CHUNK : MATE_ANY)>, p, st)
+#define RL_QK(g, u)                                                                                       \
+  (interleaved    ? qk_rope_kernel<g, MATE_NEIGHBOUR, u>                                                  \
+   : rot == 16 * g ? qk_rope_kernel<g, MATE_OTHER_CHUNK, u>                                               \
+                   : qk_rope_kernel<g, (g == 1 ? MATE_OTHER_CHUNK : MATE_ANY), u>)
+#define RL_CALL(g) (p.steps == 1 ? launch_rows(RL_QK(g, 1), qk_rope_warps(1), p, st) : launch_rows(RL_QK(g, 2), qk_rope_warps(2), p, st))
   RL_BY_LANES(G, RL_CALL)
 #undef RL_CALL
+#undef RL_QK
 }
 
-int rl_kv_cache_write_e4m3(const void* k, const void* v, const void* slots, int slots_i64, void* k_codes, float* k_scale,
-                           void* v_codes, float* v_scale, int T, int H, int D, int num_pages, int page_size, int64_t k_t,
-                           int64_t k_h, int64_t v_t, int64_t v_h, int64_t code_page, int64_t code_token, int64_t code_head,
-                           int64_t scale_page, int64_t scale_token, int64_t scale_head, void* stream) {
+int rl_kv_cache_write_e4m3(const rl_kv_cache_write_args* args, void* stream) {
+  if (!args) return RL_ERR_NULL_POINTER;
+  const auto [cache, k, v, slots, T64, k_t, k_h, v_t, v_h, slots_i64] = *args;
   if (!k || !v || !slots) return RL_ERR_NULL_POINTER;
   KvWriteParams p{};
-  p.c = KvCache{(uint8_t*)k_codes, (uint8_t*)v_codes, k_scale, v_scale, code_page, code_token, code_head,
-                scale_page, scale_token, scale_head, num_pages, page_size, H, D};
-  int rc = check_cache(p.c);
+  int rc = check_cache(cache, &p.c);
   if (rc) return rc;
+  if (!fit_int({T64})) return RL_ERR_BAD_SHAPE;
+  const int T = (int)T64, H = p.c.H, D = p.c.D;
   if (T <= 0 || H > 32768 || !nonneg({k_t, k_h, v_t, v_h})) return RL_ERR_BAD_SHAPE;
   if (!aligned16(k) || !aligned16(v) || !mult8({k_t, k_h, v_t, v_h}) ||
       (reinterpret_cast<uintptr_t>(slots) & (slots_i64 ? 7 : 3)))
     return RL_ERR_ALIGNMENT;
-  const View kc = code_view(p.c, k_codes), vc = code_view(p.c, v_codes), ks = scale_view(p.c, k_scale), vs = scale_view(p.c, v_scale);
+  const View kc = code_view(p.c, p.c.k_codes), vc = code_view(p.c, p.c.v_codes), ks = scale_view(p.c, p.c.k_scale),
+             vs = scale_view(p.c, p.c.v_scale);
   const View vk = head_view(k, T, H, D, k_t, k_h), vv = head_view(v, T, H, D, v_t, v_h), vsl(slots, slots_i64 ? 8 : 4, {{T, 1}});
   if (kc.self_overlaps() || ks.self_overlaps() || !disjoint(kc, vc) || !disjoint(ks, vs) || !disjoint(kc, ks) ||
       !disjoint(kc, vs) || !disjoint(vc, ks) || !disjoint(vc, vs))
@@ -1285,32 +1299,31 @@ int rl_kv_cache_write_e4m3(const void* k, const void* v, const void* slots, int 
   if (di.cc_major != 10) return RL_ERR_UNSUPPORTED_ARCH;
   p.k = reinterpret_cast<const __nv_bfloat16*>(k); p.v = reinterpret_cast<const __nv_bfloat16*>(v);
   p.k_t = k_t; p.k_h = k_h; p.v_t = v_t; p.v_h = v_h;
-  p.slots = slots; p.slots64 = slots_i64; p.T = T;
+  p.slots = slots; p.slots64 = slots_i64 != 0; p.T = T;
   const int G = lanes_per_row(D), groups = 2 * ((H + 32 / G - 1) / (32 / G));
   p.steps = pick_steps(T, groups, di.sms);
   p.parts = (groups + p.steps - 1) / p.steps;
-#define RL_CALL(g) launch_rows(kv_write_kernel<g>, p, (cudaStream_t)stream)
+#define RL_CALL(g) launch_rows(p.steps == 1 ? kv_write_kernel<g, 1> : kv_write_kernel<g, 2>, KV_WARPS, p, (cudaStream_t)stream)
   RL_BY_LANES(G, RL_CALL)
 #undef RL_CALL
 }
 
-int rl_kv_cache_read_e4m3(const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
-                          const int* page_table, const int* cu_seqlens, void* k_out, void* v_out, int total, int zero_tail,
-                          int B, int max_pages, int64_t ld_pages, int H, int D, int num_pages, int page_size, int64_t code_page,
-                          int64_t code_token, int64_t code_head, int64_t scale_page, int64_t scale_token, int64_t scale_head,
-                          int64_t ko_t, int64_t ko_h, int64_t vo_t, int64_t vo_h, void* stream) {
-  if (!k_out || !v_out || !cu_seqlens || (!page_table && B > 0 && max_pages > 0)) return RL_ERR_NULL_POINTER;
+int rl_kv_cache_read_e4m3(const rl_kv_cache_read_args* args, void* stream) {
+  if (!args) return RL_ERR_NULL_POINTER;
+  const auto [cache, page_table, cu_seqlens, k_out, v_out, total64, zero_tail, B64, max_pages64, ld_pages, ko_t, ko_h, vo_t, vo_h] = *args;
+  if (!k_out || !v_out || !cu_seqlens || (!page_table && B64 > 0 && max_pages64 > 0)) return RL_ERR_NULL_POINTER;
   KvReadParams p{};
-  p.c = KvCache{(uint8_t*)k_codes, (uint8_t*)v_codes, (float*)k_scale, (float*)v_scale, code_page, code_token, code_head,
-                scale_page, scale_token, scale_head, num_pages, page_size, H, D};
-  int rc = check_cache(p.c);
+  int rc = check_cache(cache, &p.c);
   if (rc) return rc;
+  if (!fit_int({total64, B64, max_pages64})) return RL_ERR_BAD_SHAPE;
+  const int total = (int)total64, B = (int)B64, max_pages = (int)max_pages64, H = p.c.H, D = p.c.D;
   if (total <= 0 || B < 0 || max_pages < 0 || ld_pages < 0 || H > 32768 || !nonneg({ko_t, ko_h, vo_t, vo_h})) return RL_ERR_BAD_SHAPE;
   if (!aligned16(k_out) || !aligned16(v_out) || !mult8({ko_t, ko_h, vo_t, vo_h}) ||
       ((reinterpret_cast<uintptr_t>(page_table) | reinterpret_cast<uintptr_t>(cu_seqlens)) & 3))
     return RL_ERR_ALIGNMENT;
   const View vko = head_view(k_out, total, H, D, ko_t, ko_h), vvo = head_view(v_out, total, H, D, vo_t, vo_h);
-  const View kc = code_view(p.c, k_codes), vc = code_view(p.c, v_codes), ks = scale_view(p.c, k_scale), vs = scale_view(p.c, v_scale);
+  const View kc = code_view(p.c, p.c.k_codes), vc = code_view(p.c, p.c.v_codes), ks = scale_view(p.c, p.c.k_scale),
+             vs = scale_view(p.c, p.c.v_scale);
   const View vt(page_table, 4, {{B, ld_pages}, {max_pages, 1}}), vcu(cu_seqlens, 4, {{(int64_t)B + 1, 1}});
   if (vko.self_overlaps() || vvo.self_overlaps() || !disjoint(vko, vvo)) return RL_ERR_OVERLAP;
   for (const View* o : {&vko, &vvo})
@@ -1320,13 +1333,13 @@ int rl_kv_cache_read_e4m3(const void* k_codes, const float* k_scale, const void*
   if ((rc = device_info(&di))) return rc;
   if (di.cc_major != 10) return RL_ERR_UNSUPPORTED_ARCH;
   p.pages = page_table; p.ld_pages = ld_pages; p.cu = cu_seqlens; p.B = B; p.max_pages = max_pages;
-  p.T = total; p.zero_tail = zero_tail;
+  p.T = total; p.zero_tail = zero_tail != 0;
   p.k_out = reinterpret_cast<__nv_bfloat16*>(k_out); p.v_out = reinterpret_cast<__nv_bfloat16*>(v_out);
   p.ko_t = ko_t; p.ko_h = ko_h; p.vo_t = vo_t; p.vo_h = vo_h;
   const int G = lanes_per_row(D), groups = 2 * ((H + 32 / G - 1) / (32 / G));
   p.steps = pick_steps(total, groups, di.sms);
   p.parts = (groups + p.steps - 1) / p.steps;
-#define RL_CALL(g) launch_rows(kv_read_kernel<g>, p, (cudaStream_t)stream)
+#define RL_CALL(g) launch_rows(kv_read_kernel<g>, KV_WARPS, p, (cudaStream_t)stream)
   RL_BY_LANES(G, RL_CALL)
 #undef RL_CALL
 }

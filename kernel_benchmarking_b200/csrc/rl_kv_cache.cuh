@@ -13,6 +13,8 @@
 
 namespace rl {
 
+constexpr int KV_WARPS = 4;  // per block
+
 struct KvCache {           // codes [pages, page_size, H, D], scales [pages, page_size, H]; values laid out like keys
   uint8_t *k_codes, *v_codes;
   float *k_scale, *v_scale;
@@ -46,30 +48,20 @@ __device__ __forceinline__ uint2 e4m3_codes(const uint32_t (&xs)[4], float inv) 
   return make_uint2(code[0] | (code[1] << 16), code[2] | (code[3] << 16));
 }
 
-template <int G>
-__global__ void __launch_bounds__(128) kv_write_kernel(const KvWriteParams p) {
+// U: groups whose loads are in flight together
+template <int G, int U>
+__global__ void __launch_bounds__(32 * KV_WARPS) kv_write_kernel(const KvWriteParams p) {
   constexpr int R = 32 / G;
-  constexpr int U = 2;  // groups whose loads are in flight together
   launch_dependents();
   grid_dependency_wait();
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const long long w = (long long)blockIdx.x * KV_WARPS + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, c = lane & (G - 1);
   const int t = (int)(w / p.parts), part = (int)(w - (long long)t * p.parts);
   if (t >= p.T) return;
-  const long long slot = load_index(p.slots, t, p.slots64);
-  if (slot < 0) return;
-  const long long page = slot / p.c.page_size;
-  const int off = (int)(slot - page * p.c.page_size);
-  if (page >= p.c.num_pages) {
-    if (lane == 0 && part == 0) record_bad_index(BAD_SLOT, t, slot);
-    return;
-  }
-  const long long code_at = page * p.c.c_page + off * p.c.c_off, scale_at = page * p.c.s_page + off * p.c.s_off;
   const int k_groups = (p.c.H + R - 1) / R;  // the key heads' groups, then as many of the value heads
   const int g0 = part * p.steps, g1 = min(g0 + p.steps, 2 * k_groups);
-#pragma unroll 1
-  for (int g = g0; g < g1; g += U) {
-    uint32_t x[U][2][4];
+  uint32_t x[U][2][4];
+  auto load_rows = [&](int g) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool is_k = g + u < k_groups;
@@ -83,6 +75,20 @@ __global__ void __launch_bounds__(128) kv_write_kernel(const KvWriteParams p) {
         x[u][j][0] = v.x; x[u][j][1] = v.y; x[u][j][2] = v.z; x[u][j][3] = v.w;
       }
     }
+  };
+  load_rows(g0);  // on their way while the slot is looked up
+  const long long slot = load_index(p.slots, t, p.slots64);
+  if (slot < 0) return;
+  const long long page = slot / p.c.page_size;
+  const int off = (int)(slot - page * p.c.page_size);
+  if (page >= p.c.num_pages) {
+    if (lane == 0 && part == 0) record_bad_index(BAD_SLOT, t, slot);
+    return;
+  }
+  const long long code_at = page * p.c.c_page + off * p.c.c_off, scale_at = page * p.c.s_page + off * p.c.s_off;
+#pragma unroll 1
+  for (int g = g0; g < g1; g += U) {
+    if (g > g0) load_rows(g);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool is_k = g + u < k_groups;
@@ -147,12 +153,12 @@ __device__ __forceinline__ uint32_t dequant2(uint32_t codes, float scale) {
 }
 
 template <int G>
-__global__ void __launch_bounds__(128) kv_read_kernel(const KvReadParams p) {
+__global__ void __launch_bounds__(32 * KV_WARPS) kv_read_kernel(const KvReadParams p) {
   constexpr int R = 32 / G;
   constexpr int U = 4;  // groups whose loads are in flight together
   launch_dependents();
   grid_dependency_wait();
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const long long w = (long long)blockIdx.x * KV_WARPS + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, c = lane & (G - 1);
   const int i = (int)(w / p.parts), part = (int)(w - (long long)i * p.parts);
   if (i >= p.T) return;

@@ -10,13 +10,15 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _status_devices, _raw_stream
+from .ops import _raw_stream, _status_devices
+
+_BF16, _E4M3 = torch.bfloat16, torch.float8_e4m3fn
 
 
 # The checks sit on the path of every decode step, whose kernels run for a few microseconds: each call makes them as one
 # plain condition first and looks for what is wrong, and the words for it, only when that fails.
 
-def _explain_heads(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> None:
+def _explain_heads(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
     """[tokens, heads, channels] bf16 on the GPU, channels contiguous; the strides of tokens and heads are free."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -26,34 +28,38 @@ def _explain_heads(name: str, t: torch.Tensor, device: Optional[torch.device] = 
         raise ValueError(f"{name} must be torch.bfloat16, got {t.dtype}")
     if t.dim() != 3 or t.stride(2) != 1:
         raise ValueError(f"{name} must be [tokens, heads, channels] with contiguous channels, got {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}, got {t.device}")
 
 
 def _heads_ok(t: torch.Tensor, dev: int) -> bool:
-    return (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.get_device() == dev and t.dim() == 3
-            and t.stride(2) == 1)
+    if not isinstance(t, torch.Tensor):
+        return False
+    strides = t.stride()
+    return t.dtype is _BF16 and t.get_device() == dev and len(strides) == 3 and strides[2] == 1
 
 
 def _index_ok(t: torch.Tensor, n: int, dev: int) -> bool:
     """A contiguous vector of n int64 or int32."""
     return (isinstance(t, torch.Tensor) and (t.dtype is torch.int64 or t.dtype is torch.int32) and t.get_device() == dev
-            and t.dim() == 1 and t.shape[0] == n and (t.stride(0) == 1 or n <= 1))
+            and t.shape == (n,) and t.is_contiguous())
 
 
-def _gamma_ok(g: Optional[torch.Tensor], D: int, dev: int) -> bool:
-    return g is None or (isinstance(g, torch.Tensor) and g.dtype is torch.bfloat16 and g.get_device() == dev
-                         and g.shape == (D,) and (g.stride(0) == 1 or D <= 1))
+def _gamma_ok(g: torch.Tensor, D: int, dev: int) -> bool:
+    return (isinstance(g, torch.Tensor) and g.dtype is _BF16 and g.get_device() == dev and g.shape == (D,)
+            and g.is_contiguous())
 
 
-def _call(dev: int, fn, *args) -> int:
-    """The C function with the device's current stream behind the arguments, on that device."""
+def _call(what: str, fn, args: bytes, dev: int) -> None:
+    """The C function on the device, and on its current stream."""
     if dev == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(dev))
+        rc = fn(args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
-    return rc
+            rc = fn(args, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
+    _status_devices.add(dev)
 
 
 def rope_table(positions: int, rotary_dim: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:
@@ -77,18 +83,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: Optional[torch.Tenso
     `positions` [T] int64 or int32; one outside the table leaves its token's rows unwritten and `check_status` raises.
     D a multiple of 8 up to 256, rotary_dim of 16 (interleaved: 8).  `out`: a pair of tensors to write, q and k
     themselves for an update in place; they may share no other memory with the inputs or each other."""
-    dev = q.get_device() if isinstance(q, torch.Tensor) and q.is_cuda else None
-    if dev is None or not (_heads_ok(q, dev) and _heads_ok(k, dev)):
+    dev = q.get_device() if isinstance(q, torch.Tensor) else -1
+    if dev < 0 or not _heads_ok(q, dev) or not _heads_ok(k, dev):
         _explain_heads("q", q)
-        _explain_heads("k", k, q.device)
+        _explain_heads("k", k, q)
     T, Hq, D = q.shape
     Tk, Hk, Dk = k.shape
     if Tk != T or Dk != D:
         raise ValueError(f"q is [{T}, {Hq}, {D}]: k must be [{T}, Hk, {D}], got {tuple(k.shape)}")
-    if not (_gamma_ok(q_gamma, D, dev) and _gamma_ok(k_gamma, D, dev)):
+    if (q_gamma is not None and not _gamma_ok(q_gamma, D, dev)) or (k_gamma is not None and not _gamma_ok(k_gamma, D, dev)):
         raise ValueError(f"q_gamma and k_gamma must be contiguous bf16 vectors of length D={D} on q's device")
-    if (not isinstance(table, torch.Tensor) or table.dtype is not torch.float32 or table.dim() != 2
-            or table.get_device() != dev or table.stride(1) != 1):
+    table_strides = table.stride() if isinstance(table, torch.Tensor) else ()
+    if len(table_strides) != 2 or table_strides[1] != 1 or table.dtype is not torch.float32 or table.get_device() != dev:
         raise ValueError("table must be [positions, rotary_dim] fp32, row-major, on q's device")
     if not _index_ok(positions, T, dev):
         raise ValueError(f"positions must be a contiguous vector of {T} int64 or int32 on q's device")
@@ -98,8 +104,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: Optional[torch.Tenso
     else:
         qo, ko = out
         if not (_heads_ok(qo, dev) and _heads_ok(ko, dev)):
-            _explain_heads("out[0]", qo, q.device)
-            _explain_heads("out[1]", ko, q.device)
+            _explain_heads("out[0]", qo, q)
+            _explain_heads("out[1]", ko, q)
         if qo.shape != q.shape or ko.shape != k.shape:
             raise ValueError(f"out must be {tuple(q.shape)} and {tuple(k.shape)}, got {tuple(qo.shape)} and {tuple(ko.shape)}")
     if T == 0:
@@ -109,37 +115,27 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: Optional[torch.Tenso
     k_t, k_h, _ = k.stride()
     qo_t, qo_h, _ = qo.stride()
     ko_t, ko_h, _ = ko.stride()
-    rc = _call(dev, _lib.load().rl_qk_norm_rope_bf16,
-               q.data_ptr(), k.data_ptr(), None if q_gamma is None else q_gamma.data_ptr(),
-               None if k_gamma is None else k_gamma.data_ptr(), table.data_ptr(), positions.data_ptr(),
-               positions.dtype is torch.int64, qo.data_ptr(), ko.data_ptr(), T, Hq, Hk, D, rot, P, table.stride(0), q_t, q_h,
-               k_t, k_h, qo_t, qo_h, ko_t, ko_h, eps, interleaved)
-    if rc:
-        _lib.check(rc, "rl_qk_norm_rope_bf16")
-    _status_devices.add(dev)
+    _call("rl_qk_norm_rope_bf16", _lib.load().rl_qk_norm_rope_bf16, _lib.QK_NORM_ROPE_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), 0 if q_gamma is None else q_gamma.data_ptr(), 0 if k_gamma is None else k_gamma.data_ptr(),
+        table.data_ptr(), positions.data_ptr(), qo.data_ptr(), ko.data_ptr(), T, Hq, Hk, D, rot, P, table_strides[0], q_t, q_h,
+        k_t, k_h, qo_t, qo_h, ko_t, ko_h, positions.dtype is torch.int64, interleaved, eps), dev)
     return qo, ko
 
 
-def _cache_ok(k_codes, k_scale, v_codes, v_scale, dev: int) -> bool:
-    shape, strides = k_codes.shape, k_codes.stride()
-    return (k_codes.dtype is torch.float8_e4m3fn and v_codes.dtype is torch.float8_e4m3fn and k_scale.dtype is torch.float32
-            and v_scale.dtype is torch.float32 and v_codes.get_device() == dev and k_scale.get_device() == dev
-            and v_scale.get_device() == dev and len(shape) == 4 and strides[3] == 1 and v_codes.shape == shape
-            and v_codes.stride() == strides and k_scale.shape == shape[:3] and v_scale.shape == shape[:3]
-            and v_scale.stride() == k_scale.stride())
-
-
-def _check_cache(k_codes, k_scale, v_codes, v_scale) -> int:
-    """Returns the cache's device index."""
+def _check_cache(k_codes, k_scale, v_codes, v_scale) -> Tuple[int, tuple]:
+    """The cache's device index, and its part of the C structures (without a copy of anything)."""
     named = (("k_codes", k_codes), ("k_scale", k_scale), ("v_codes", v_codes), ("v_scale", v_scale))
     for name, t in named:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
-    dev = k_codes.get_device()
-    if dev >= 0 and _cache_ok(k_codes, k_scale, v_codes, v_scale, dev):
-        return dev
+    dev, shape, c, s = k_codes.get_device(), k_codes.shape, k_codes.stride(), k_scale.stride()
+    if (dev >= 0 and len(c) == 4 and c[3] == 1 and len(s) == 3 and k_codes.dtype is _E4M3 and v_codes.dtype is _E4M3
+            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and v_codes.get_device() == dev
+            and k_scale.get_device() == dev and v_scale.get_device() == dev and v_codes.shape == shape
+            and v_codes.stride() == c and k_scale.shape == shape[:3] and v_scale.shape == shape[:3] and v_scale.stride() == s):
+        return dev, (k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *shape, c[0], c[1], c[2], *s)
     for name, t in named:
-        dtype, nd = (torch.float8_e4m3fn, 4) if name.endswith("codes") else (torch.float32, 3)
+        dtype, nd = (_E4M3, 4) if name.endswith("codes") else (torch.float32, 3)
         if not t.is_cuda:
             raise ValueError(f"{name} must be a CUDA tensor (this operator has no CPU path)")
         if t.dtype != dtype or t.dim() != nd or t.device != k_codes.device:
@@ -160,29 +156,21 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_code
     channels, the same for keys and values.  `slots` [T] int64 or int32: page * page_size + place in the page.  Negative:
     a padding token, left out.  Beyond the cache: left out, and `check_status` raises.  The slots of one call must differ.
     A NaN stays NaN; a row with an infinity reads back as NaN throughout.  D a multiple of 8 up to 256."""
-    dev = _check_cache(k_codes, k_scale, v_codes, v_scale)
+    dev, cache = _check_cache(k_codes, k_scale, v_codes, v_scale)
     if not (_heads_ok(k, dev) and _heads_ok(v, dev)):
-        _explain_heads("k", k, k_codes.device)
-        _explain_heads("v", v, k_codes.device)
+        _explain_heads("k", k, k_codes)
+        _explain_heads("v", v, k_codes)
     T, H, D = k.shape
-    pages, page_size, Hc, Dc = k_codes.shape
-    if v.shape != k.shape or Hc != H or Dc != D:
-        raise ValueError(f"k and v must be [T, {Hc}, {Dc}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if v.shape != k.shape or cache[6] != H or cache[7] != D:
+        raise ValueError(f"k and v must be [T, {cache[6]}, {cache[7]}], got {tuple(k.shape)} and {tuple(v.shape)}")
     if not _index_ok(slots, T, dev):
         raise ValueError(f"slots must be a contiguous vector of {T} int64 or int32 on the cache's device")
     if T == 0:
         return
-    c_page, c_off, c_head, _ = k_codes.stride()
-    s_page, s_off, s_head = k_scale.stride()
     k_t, k_h, _ = k.stride()
     v_t, v_h, _ = v.stride()
-    rc = _call(dev, _lib.load().rl_kv_cache_write_e4m3,
-               k.data_ptr(), v.data_ptr(), slots.data_ptr(), slots.dtype is torch.int64, k_codes.data_ptr(),
-               k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), T, H, D, pages, page_size, k_t, k_h, v_t, v_h,
-               c_page, c_off, c_head, s_page, s_off, s_head)
-    if rc:
-        _lib.check(rc, "rl_kv_cache_write_e4m3")
-    _status_devices.add(dev)
+    _call("rl_kv_cache_write_e4m3", _lib.load().rl_kv_cache_write_e4m3, _lib.KV_CACHE_WRITE_ARGS.pack(
+        *cache, k.data_ptr(), v.data_ptr(), slots.data_ptr(), T, k_t, k_h, v_t, v_h, slots.dtype is torch.int64), dev)
 
 
 def kv_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
@@ -195,10 +183,11 @@ def kv_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.T
     `total` is the caller's: rows from cu_seqlens[B] on are zero in a fresh output and left as they are in `out`,
     tokens beyond `total` are not read.  A page outside the cache (or a sequence longer than its table row) leaves the
     row as it is, unspecified in a fresh output, and `check_status` raises."""
-    dev = _check_cache(k_codes, k_scale, v_codes, v_scale)
-    pages, page_size, H, D = k_codes.shape
-    if (not isinstance(page_table, torch.Tensor) or page_table.dtype is not torch.int32 or page_table.dim() != 2
-            or page_table.get_device() != dev or (page_table.stride(1) != 1 and page_table.shape[1] > 1)):
+    dev, cache = _check_cache(k_codes, k_scale, v_codes, v_scale)
+    H, D = cache[6], cache[7]
+    strides = page_table.stride() if isinstance(page_table, torch.Tensor) else ()
+    if (len(strides) != 2 or page_table.dtype is not torch.int32 or page_table.get_device() != dev
+            or (strides[1] != 1 and page_table.shape[1] > 1)):
         raise ValueError("page_table must be [B, max_pages] int32, row-major, on the cache's device")
     B, max_pages = page_table.shape
     if not _index_ok(cu_seqlens, B + 1, dev) or cu_seqlens.dtype is not torch.int32:
@@ -206,26 +195,20 @@ def kv_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.T
     if total < 0:
         raise ValueError("total must not be negative")
     if out is None:
-        ko = k_codes.new_empty((total, H, D), dtype=torch.bfloat16)
-        vo = k_codes.new_empty((total, H, D), dtype=torch.bfloat16)
+        ko = k_codes.new_empty((total, H, D), dtype=_BF16)
+        vo = torch.empty_like(ko)
     else:
         ko, vo = out
         if not (_heads_ok(ko, dev) and _heads_ok(vo, dev)):
-            _explain_heads("out[0]", ko, k_codes.device)
-            _explain_heads("out[1]", vo, k_codes.device)
+            _explain_heads("out[0]", ko, k_codes)
+            _explain_heads("out[1]", vo, k_codes)
         if ko.shape != (total, H, D) or vo.shape != ko.shape:
             raise ValueError(f"out must be two tensors [{total}, {H}, {D}], got {tuple(ko.shape)} and {tuple(vo.shape)}")
     if total == 0:
         return ko, vo
-    c_page, c_off, c_head, _ = k_codes.stride()
-    s_page, s_off, s_head = k_scale.stride()
     ko_t, ko_h, _ = ko.stride()
     vo_t, vo_h, _ = vo.stride()
-    rc = _call(dev, _lib.load().rl_kv_cache_read_e4m3,
-               k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), page_table.data_ptr(),
-               cu_seqlens.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, out is None, B, max_pages, page_table.stride(0),
-               H, D, pages, page_size, c_page, c_off, c_head, s_page, s_off, s_head, ko_t, ko_h, vo_t, vo_h)
-    if rc:
-        _lib.check(rc, "rl_kv_cache_read_e4m3")
-    _status_devices.add(dev)
+    _call("rl_kv_cache_read_e4m3", _lib.load().rl_kv_cache_read_e4m3, _lib.KV_CACHE_READ_ARGS.pack(
+        *cache, page_table.data_ptr(), cu_seqlens.data_ptr(), ko.data_ptr(), vo.data_ptr(), total, out is None, B, max_pages,
+        strides[0], ko_t, ko_h, vo_t, vo_h), dev)
     return ko, vo

@@ -22,10 +22,12 @@ _status_devices: set = set()  # devices on which a kernel without a workspace ha
 _CLEAN_BYTES = 256 + 65536   # status block and tile counters: the part of a workspace that starts from zero
 
 
-def _raw_stream(idx: int) -> int:
-    """Raw handle of torch's current stream on device `idx` (the fast C accessor when torch has it)."""
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(idx) if raw is not None else torch.cuda.current_stream(idx).cuda_stream
+def _stream_of(idx: int) -> int:
+    return torch.cuda.current_stream(idx).cuda_stream
+
+
+# raw handle of torch's current stream on a device (the fast C accessor when torch has it)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream_of)
 
 
 def _stream_ptr(device: Optional[torch.device] = None) -> int:
@@ -251,8 +253,10 @@ def _linear_workspace_bytes(M: int, N: int, K: int) -> int:
 
 
 def _matrix_ok(t: torch.Tensor, dev: int) -> bool:
-    return (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.get_device() == dev and t.dim() == 2
-            and t.stride(1) == 1)
+    if not isinstance(t, torch.Tensor):
+        return False
+    strides = t.stride()
+    return t.dtype is torch.bfloat16 and t.get_device() == dev and len(strides) == 2 and strides[1] == 1
 
 
 def linear_workspace(M: int, N: int, K: int, device: Optional[torch.device] = None) -> torch.Tensor:
@@ -280,8 +284,8 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
     captured into a CUDA graph takes a workspace of its own from the graph's memory and clears it on every replay, so
     graphs share none; a `linear_workspace` passed in saves that step."""
     # one plain condition on the path of every decode step; what is wrong is looked for only when it fails
-    dev = x.get_device() if isinstance(x, torch.Tensor) and x.is_cuda else None
-    if dev is None or not (_matrix_ok(x, dev) and _matrix_ok(W, dev) and (residual is None or _matrix_ok(residual, dev))):
+    dev = x.get_device() if isinstance(x, torch.Tensor) else -1
+    if dev < 0 or not (_matrix_ok(x, dev) and _matrix_ok(W, dev) and (residual is None or _matrix_ok(residual, dev))):
         _check_matrix("x", x, torch.bfloat16)
         _check_matrix("W", W, torch.bfloat16)
         if residual is not None:
@@ -292,7 +296,7 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
     if K2 != K:
         raise ValueError(f"x is [M, {K}]: W must be [N, {K}], got {tuple(W.shape)}")
     if bias is not None and not (isinstance(bias, torch.Tensor) and bias.dtype is torch.bfloat16 and bias.get_device() == dev
-                                 and bias.shape == (N,) and (bias.stride(0) == 1 or N <= 1)):
+                                 and bias.shape == (N,) and bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous bf16 vector of length N={N} on x's device")
     if residual is not None and residual.shape != (M, N):
         raise ValueError(f"residual must be [{M}, {N}], got {tuple(residual.shape)}")

@@ -1,6 +1,4 @@
 """What the linear layer, the query/key norm with rotation and the e4m3 cache refuse, before anything touches a device."""
-import ctypes
-
 import pytest
 import torch
 
@@ -77,15 +75,16 @@ def test_linear_workspace_bytes(lib):
 
 def call_qk(lib, q=A[0], k=A[1], gq=A[2], gk=A[3], table=A[4], pos=A[5], p64=1, qo=A[6], ko=A[7], T=64, Hq=8, Hk=2, D=64, rot=64,
             P=128, ldt=64, qt=512, qh=64, kt=128, kh=64, qot=512, qoh=64, kot=128, koh=64, inter=0):
-    return lib.rl_qk_norm_rope_bf16(q, k, gq, gk, table, pos, p64, qo, ko, T, Hq, Hk, D, rot, P, ldt, qt, qh, kt, kh, qot, qoh,
-                                    kot, koh, ctypes.c_float(1e-6), inter, None)
+    return lib.rl_qk_norm_rope_bf16(_lib.QK_NORM_ROPE_ARGS.pack(
+        *(p or 0 for p in (q, k, gq, gk, table, pos, qo, ko)), T, Hq, Hk, D, rot, P, ldt, qt, qh, kt, kh, qot, qoh, kot, koh, p64,
+        inter, 1e-6), None)
 
 
 @pytest.mark.parametrize("rc,kw", [
     (N_ERR, dict(q=None)), (N_ERR, dict(k=None)), (N_ERR, dict(table=None)), (N_ERR, dict(pos=None)), (N_ERR, dict(qo=None)),
     (N_ERR, dict(ko=None)),
     (SHAPE, dict(T=0)), (SHAPE, dict(Hq=0)), (SHAPE, dict(Hk=0)), (SHAPE, dict(D=264)), (SHAPE, dict(rot=0)), (SHAPE, dict(rot=80)),
-    (SHAPE, dict(P=-1)), (SHAPE, dict(ldt=60)), (SHAPE, dict(qh=-64)),
+    (SHAPE, dict(P=-1)), (SHAPE, dict(T=2 ** 31)), (SHAPE, dict(P=2 ** 32)), (SHAPE, dict(ldt=60)), (SHAPE, dict(qh=-64)),
     (ALIGN, dict(D=60, rot=48)), (ALIGN, dict(rot=56)), (ALIGN, dict(rot=60, inter=1)), (ALIGN, dict(qt=516)),
     (ALIGN, dict(koh=68)), (ALIGN, dict(ldt=66)), (ALIGN, dict(q=A[0] + 8)), (ALIGN, dict(gk=A[3] + 2)),
     (ALIGN, dict(pos=A[5] + 4)), (ALIGN, dict(pos=A[5] + 2, p64=0)),
@@ -114,13 +113,14 @@ def test_qk_norm_rope_accepts(lib):
 
 def call_write(lib, k=A[0], v=A[1], slots=A[2], s64=1, kc=A[3], ks=A[4], vc=A[5], vs=A[6], T=64, H=8, D=64, pages=32, page=16,
                kt=512, kh=64, vt=512, vh=64, cp=8192, co=512, ch=64, sp=128, so=8, sh=1):
-    return lib.rl_kv_cache_write_e4m3(k, v, slots, s64, kc, ks, vc, vs, T, H, D, pages, page, kt, kh, vt, vh, cp, co, ch, sp, so,
-                                      sh, None)
+    return lib.rl_kv_cache_write_e4m3(_lib.KV_CACHE_WRITE_ARGS.pack(
+        *(p or 0 for p in (kc, vc, ks, vs)), pages, page, H, D, cp, co, ch, sp, so, sh, *(p or 0 for p in (k, v, slots)), T, kt, kh,
+        vt, vh, s64), None)
 
 
 @pytest.mark.parametrize("rc,kw", [
     (N_ERR, dict(k=None)), (N_ERR, dict(v=None)), (N_ERR, dict(slots=None)), (N_ERR, dict(kc=None)), (N_ERR, dict(vs=None)),
-    (SHAPE, dict(T=0)), (SHAPE, dict(H=0)), (SHAPE, dict(D=264)), (SHAPE, dict(page=0)), (SHAPE, dict(pages=-1)),
+    (SHAPE, dict(T=0)), (SHAPE, dict(H=0)), (SHAPE, dict(D=264)), (SHAPE, dict(page=0)), (SHAPE, dict(pages=-1)), (SHAPE, dict(pages=2 ** 32 + 1)), (SHAPE, dict(T=2 ** 32 + 1)),
     (SHAPE, dict(kt=-512)), (SHAPE, dict(cp=-8192)),
     (ALIGN, dict(D=60)), (ALIGN, dict(kt=516)), (ALIGN, dict(vh=68)), (ALIGN, dict(co=516)), (ALIGN, dict(k=A[0] + 8)),
     (ALIGN, dict(kc=A[3] + 4)), (ALIGN, dict(ks=A[4] + 2)), (ALIGN, dict(slots=A[2] + 4)),
@@ -142,8 +142,9 @@ def test_kv_cache_write_accepts(lib):
 
 def call_read(lib, kc=A[0], ks=A[1], vc=A[2], vs=A[3], table=A[4], cu=A[5], ko=A[6], vo=A[7], total=64, zero=0, B=4, most=8, ldp=8,
               H=8, D=64, pages=32, page=16, cp=8192, co=512, ch=64, sp=128, so=8, sh=1, kt=512, kh=64, vt=512, vh=64):
-    return lib.rl_kv_cache_read_e4m3(kc, ks, vc, vs, table, cu, ko, vo, total, zero, B, most, ldp, H, D, pages, page, cp, co, ch,
-                                     sp, so, sh, kt, kh, vt, vh, None)
+    return lib.rl_kv_cache_read_e4m3(_lib.KV_CACHE_READ_ARGS.pack(
+        *(p or 0 for p in (kc, vc, ks, vs)), pages, page, H, D, cp, co, ch, sp, so, sh, *(p or 0 for p in (table, cu, ko, vo)), total,
+        zero, B, most, ldp, kt, kh, vt, vh), None)
 
 
 @pytest.mark.parametrize("rc,kw", [
@@ -162,6 +163,13 @@ def test_kv_cache_read_accepts(lib):
     assert passed(call_read(lib))
     assert passed(call_read(lib, B=0, table=None))
     assert passed(call_read(lib, vo=A[6] + 1024, kt=1024, vt=1024))    # keys and values of a token side by side
+
+
+def test_argument_structures(lib):
+    """The packed formats are the header's structures: pointers and 64-bit integers, no padding."""
+    assert _lib.QK_NORM_ROPE_ARGS.size == 8 * 26 and _lib.KV_CACHE_WRITE_ARGS.size == 8 * 23 and _lib.KV_CACHE_READ_ARGS.size == 8 * 27
+    for f in (lib.rl_qk_norm_rope_bf16, lib.rl_kv_cache_write_e4m3, lib.rl_kv_cache_read_e4m3):
+        assert f(None, None) == N_ERR
 
 
 def test_new_error_strings(lib):
