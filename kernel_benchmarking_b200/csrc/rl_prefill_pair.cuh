@@ -853,6 +853,10 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_const
 #pragma unroll 1
           for (int c = 0; c < nch; ++c) {
             uint8_t* stage = smem + Cfg::OFF_EPI + (c & 1) * Cfg::EPI_BYTES;
+            if (c >= 2) {  // (512-column tiles) the store of the chunk before last must have read its staging tile
+              if (epi_tid == 0) tma_store_wait_read<1>();
+              named_bar_sync(1, 128);
+            }
             uint32_t o[2][16];
 #pragma unroll
             for (int qq = 0; qq < 4; ++qq) {  // 16 columns at a time keeps the register count of the hot loops
