@@ -231,9 +231,12 @@ int rl_lora_linear_bf16(const void* a, const void* b, const void* xa, const void
  *   variant: RL_VARIANT_AUTO or RL_VARIANT_AUTO_WHOLE (see Concurrency above).
  * No reference counterpart beyond its plain GEMM (demo/new_profiling/rmsnorm_linear_new.py:29-31). */
 size_t rl_linear_workspace_bytes(int M, int N, int K);
-int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* residual, void* y, int M, int N, int K,
-                   int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int activation,
-                   void* workspace, size_t workspace_bytes, int variant, void* stream);
+typedef struct {
+  const void *x, *W, *bias, *residual;
+  void *y, *workspace;
+  int64_t M, N, K, ldx, ldw, ldr, ldy, activation, variant, workspace_bytes;
+} rl_linear_args;
+int rl_linear_bf16(const rl_linear_args* args, void* stream);
 
 /* RMSNorm of every query and key head and the rotation by position, in one pass over what the QKV projection wrote.
  *   n = x * gamma * rsqrt(mean_d x^2 + eps) over the D channels of one head, then for each pair (i, j) of the first

@@ -70,8 +70,8 @@ SYMBOLS = [
     ("rl_gemm_bf16", _i, [_vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _vp, _sz, _vp]),
     ("rl_lora_linear_bf16", _i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     ("rl_linear_workspace_bytes", _sz, [_i, _i, _i]),
-    ("rl_linear_bf16", _i, [_vp] * 5 + [_i] * 3 + [_i64] * 4 + [_i, _vp, _sz, _i, _vp]),
-    # (the arguments of these three are C structures, packed with the formats below)
+    # (the arguments of these four are C structures, packed with the formats below)
+    ("rl_linear_bf16", _i, [ctypes.c_char_p, _vp]),
     ("rl_qk_norm_rope_bf16", _i, [ctypes.c_char_p, _vp]),
     ("rl_kv_cache_write_e4m3", _i, [ctypes.c_char_p, _vp]),
     ("rl_kv_cache_read_e4m3", _i, [ctypes.c_char_p, _vp]),
@@ -80,8 +80,9 @@ SYMBOLS = [
     ("rl_read_status", _i, [_vp, ctypes.POINTER(ctypes.c_int)]),
 ]
 
-# rl_qk_norm_rope_args, rl_kv_cache_write_args, rl_kv_cache_read_args: pointers and 64-bit integers in the header's order.
+# rl_linear_args, rl_qk_norm_rope_args, rl_kv_cache_write_args, rl_kv_cache_read_args: pointers and 64-bit integers in the header's order.
 # One packed buffer costs a call 0.5 us where 30 converted arguments cost 2.5.
+LINEAR_ARGS = struct.Struct("6P10q")
 QK_NORM_ROPE_ARGS = struct.Struct("8P17qd")
 KV_CACHE_WRITE_ARGS = struct.Struct("4P10q3P6q")
 KV_CACHE_READ_ARGS = struct.Struct("4P10q4P9q")

@@ -1164,10 +1164,13 @@ size_t rl_linear_workspace_bytes(int M, int N, int K) {
   return ws_layout(M, N).tail_total;
 }
 
-int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* residual, void* y, int M, int N, int K,
-                   int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int activation, void* workspace,
-                   size_t workspace_bytes, int variant, void* stream) {
+int rl_linear_bf16(const rl_linear_args* args, void* stream) {
+  if (!args) return RL_ERR_NULL_POINTER;
+  const auto [x, W, bias, residual, y, workspace, M64, N64, K64, ldx, ldw, ldr, ldy, activation, variant, ws_bytes] = *args;
   if (!x || !W || !y) return RL_ERR_NULL_POINTER;
+  if (!fit_int({M64, N64, K64}) || ws_bytes < 0) return RL_ERR_BAD_SHAPE;
+  const int M = (int)M64, N = (int)N64, K = (int)K64;
+  const size_t workspace_bytes = (size_t)ws_bytes;
   if (M <= 0 || N <= 0 || K <= 0 || ldx < K || ldw < K || ldy < N || (residual && ldr != 0 && ldr < N))
     return RL_ERR_BAD_SHAPE;
   if (activation < RL_ACT_NONE || activation > RL_ACT_SILU) return RL_ERR_BAD_ACTIVATION;
@@ -1201,7 +1204,7 @@ int rl_linear_bf16(const void* x, const void* W, const void* bias, const void* r
   pa.split_tail = (variant != RL_VARIANT_AUTO_WHOLE);
   pa.bias = reinterpret_cast<const __nv_bfloat16*>(bias);
   pa.residual = reinterpret_cast<const __nv_bfloat16*>(residual);
-  pa.ld_res = ldr; pa.act = activation;
+  pa.ld_res = ldr; pa.act = (int)activation;
   if (plan.nt != 0) {
     switch (plan.nt) {
       case 16: return launch_split<SplitCfg<16, 6>>(pa, plan.split);

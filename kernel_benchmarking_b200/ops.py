@@ -343,10 +343,10 @@ def _launch_linear(dev, x, W, bias, residual, out, M, N, K, act, ws, nbytes, var
             ws = _workspace(x.device, nbytes, stream)
     if nbytes:
         ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
-    return lib.rl_linear_bf16(x.data_ptr(), W.data_ptr(), None if bias is None else bias.data_ptr(),
-                              None if residual is None else residual.data_ptr(), out.data_ptr(), M, N, K, x.stride(0),
-                              W.stride(0), 0 if residual is None else residual.stride(0), out.stride(0), act, ws_ptr, ws_bytes,
-                              _lib.VARIANTS[variant], stream)
+    return lib.rl_linear_bf16(_lib.LINEAR_ARGS.pack(
+        x.data_ptr(), W.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
+        out.data_ptr(), ws_ptr, M, N, K, x.stride(0), W.stride(0), 0 if residual is None else residual.stride(0), out.stride(0),
+        act, _lib.VARIANTS[variant], ws_bytes), stream)
 
 
 def quantize_rows_e4m3(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-6):

@@ -31,12 +31,13 @@ no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses
 
 def call_linear(lib, x=A[0], W=A[1], bias=A[2], res=A[3], y=A[4], M=128, N=128, K=64, ldx=64, ldw=64, ldr=128, ldy=128, act=0,
                 ws=A[5], ws_bytes=1 << 30, variant=0):
-    return lib.rl_linear_bf16(x, W, bias, res, y, M, N, K, ldx, ldw, ldr, ldy, act, ws, ws_bytes, variant, None)
+    return lib.rl_linear_bf16(_lib.LINEAR_ARGS.pack(*(p or 0 for p in (x, W, bias, res, y, ws)), M, N, K, ldx, ldw, ldr, ldy, act, variant,
+                                                    ws_bytes), None)
 
 
 @pytest.mark.parametrize("rc,kw", [
     (N_ERR, dict(x=None)), (N_ERR, dict(W=None)), (N_ERR, dict(y=None)),
-    (SHAPE, dict(M=0)), (SHAPE, dict(N=0)), (SHAPE, dict(K=0)), (SHAPE, dict(ldx=56)), (SHAPE, dict(ldw=56)),
+    (SHAPE, dict(M=0)), (SHAPE, dict(N=0)), (SHAPE, dict(K=0)), (SHAPE, dict(M=2 ** 31)), (SHAPE, dict(ws_bytes=-1)), (SHAPE, dict(ldx=56)), (SHAPE, dict(ldw=56)),
     (SHAPE, dict(ldy=120)), (SHAPE, dict(ldr=127)),
     (ALIGN, dict(K=60)), (ALIGN, dict(ldx=68)), (ALIGN, dict(ldw=68)), (ALIGN, dict(x=A[0] + 8)), (ALIGN, dict(bias=A[2] + 8)),
     (ALIGN, dict(ldy=130)), (ALIGN, dict(y=A[4] + 2)), (ALIGN, dict(res=A[3] + 1)),
@@ -167,8 +168,8 @@ def test_kv_cache_read_accepts(lib):
 
 def test_argument_structures(lib):
     """The packed formats are the header's structures: pointers and 64-bit integers, no padding."""
-    assert _lib.QK_NORM_ROPE_ARGS.size == 8 * 26 and _lib.KV_CACHE_WRITE_ARGS.size == 8 * 23 and _lib.KV_CACHE_READ_ARGS.size == 8 * 27
-    for f in (lib.rl_qk_norm_rope_bf16, lib.rl_kv_cache_write_e4m3, lib.rl_kv_cache_read_e4m3):
+    assert _lib.LINEAR_ARGS.size == 8 * 16 and _lib.QK_NORM_ROPE_ARGS.size == 8 * 26 and _lib.KV_CACHE_WRITE_ARGS.size == 8 * 23 and _lib.KV_CACHE_READ_ARGS.size == 8 * 27
+    for f in (lib.rl_linear_bf16, lib.rl_qk_norm_rope_bf16, lib.rl_kv_cache_write_e4m3, lib.rl_kv_cache_read_e4m3):
         assert f(None, None) == N_ERR
 
 
