@@ -5,9 +5,9 @@
  * Every entry point takes plain pointers and sizes; device pointers belong to
  * the caller, and every launch is asynchronous on the stream that is passed in.
  * The library never calls an allocator and keeps no pointer of the caller's; the
- * one piece of device memory it owns is the fixed 3 MiB scratch array of
- * rl_rmsnorm_linear_bf16_noalloc, which is part of the library's device image
- * (see that function).  All functions return 0 on success or a negative RL_ERR_*
+ * device memory it owns is part of its device image: the fixed 3 MiB scratch array of
+ * rl_rmsnorm_linear_bf16_noalloc (see that function) and the few words that
+ * rl_take_device_status reads.  All functions return 0 on success or a negative RL_ERR_*
  * code; nothing throws.
  *
  * Concurrency.  Calls on one stream may follow each other freely.  The large-M

@@ -771,7 +771,9 @@ bool disjoint(const View& a, const View& b, int i = 0, int j = 0, int64_t shift 
 
 // How the rows of `tokens` tokens are dealt to warps: every token has `groups` groups of 32 / G rows, a warp takes `steps`
 // of them.  As many as leave 24 warps for every SM - each then has several loads in flight and makes what it needs per
-// token once -, one where there are few rows and only latency counts.
+// token once -, one where there are few rows and only latency counts.  Measured at 16384 tokens and more, all of a token's
+// groups in one warp against half of them: norm and rotation of 10 groups 60.5 / 78 us, write of 4 groups 20.9 / 23.3, read
+// of 4 groups 126 / 141.
 inline int lanes_per_row(int D) {
   int g = 1;
   while (g * 16 < D) g *= 2;
@@ -857,9 +859,9 @@ const char* rl_error_string(int code) {
   switch (code) {
     case RL_OK: return "ok";
     case RL_ERR_NULL_POINTER: return "a required pointer is NULL";
-    case RL_ERR_BAD_SHAPE: return "M, N and K must be positive and leading dimensions must cover a row";
+    case RL_ERR_BAD_SHAPE: return "a size is not positive or out of range, or a leading dimension does not cover a row";
     case RL_ERR_ALIGNMENT:
-      return "K and the leading dimensions must be multiples of 8 elements (16 for e4m3) and pointers 16-byte aligned";
+      return "K (channels of a head) and the strides must be multiples of 8 elements (16 for e4m3) and pointers 16-byte aligned";
     case RL_ERR_BAD_DTYPE: return "unknown weight dtype";
     case RL_ERR_WORKSPACE: return "workspace missing or smaller than rl_workspace_bytes()";
     case RL_ERR_UNSUPPORTED_ARCH: return "the current device is not an sm_100 (B200) GPU";

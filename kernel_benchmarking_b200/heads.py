@@ -50,7 +50,10 @@ def _gamma_ok(g: torch.Tensor, D: int, dev: int) -> bool:
             and g.is_contiguous())
 
 
-def _call(what: str, fn, args: bytes, dev: int) -> None:
+_NEEDS = "heads of a multiple of 8 channels up to 256, strides of multiples of 8 elements, 16-byte aligned"
+
+
+def _call(what: str, fn, args: bytes, dev: int, needs: str = _NEEDS) -> None:
     """The C function on the device, and on its current stream."""
     if dev == torch.cuda.current_device():
         rc = fn(args, _raw_stream(dev))
@@ -58,7 +61,7 @@ def _call(what: str, fn, args: bytes, dev: int) -> None:
         with torch.cuda.device(dev):
             rc = fn(args, _raw_stream(dev))
     if rc:
-        _lib.check(rc, what)
+        _lib.check(rc, f"{what} (needs {needs})" if rc in (_lib.RL_ERR_BAD_SHAPE, _lib.RL_ERR_ALIGNMENT) else what)
     _status_devices.add(dev)
 
 
@@ -118,7 +121,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: Optional[torch.Tenso
     _call("rl_qk_norm_rope_bf16", _lib.load().rl_qk_norm_rope_bf16, _lib.QK_NORM_ROPE_ARGS.pack(
         q.data_ptr(), k.data_ptr(), 0 if q_gamma is None else q_gamma.data_ptr(), 0 if k_gamma is None else k_gamma.data_ptr(),
         table.data_ptr(), positions.data_ptr(), qo.data_ptr(), ko.data_ptr(), T, Hq, Hk, D, rot, P, table_strides[0], q_t, q_h,
-        k_t, k_h, qo_t, qo_h, ko_t, ko_h, positions.dtype is torch.int64, interleaved, eps), dev)
+        k_t, k_h, qo_t, qo_h, ko_t, ko_h, positions.dtype is torch.int64, interleaved, eps), dev,
+        f"{_NEEDS}; rotary_dim a multiple of {8 if interleaved else 16} up to the head's")
     return qo, ko
 
 

@@ -213,6 +213,31 @@ def test_linear_k_split_in_a_graph_and_grown_workspaces():
     assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_linear_random_shapes(seed):
+    """Sizes spread over their logarithms, so over every tile and cluster size of the plan, with every way to call it."""
+    import random
+    r = random.Random(1000 + seed)
+    for i in range(50):
+        M, N = int(math.exp(r.uniform(0, math.log(3000)))), int(math.exp(r.uniform(0, math.log(6000))))
+        K = 8 * int(math.exp(r.uniform(0, math.log(512))))
+        act, s = r.choice(ACTS), 10 * i + 7 * seed
+        x, W, b, _ = linear_inputs(M, N, K, s, r.random() < 0.5, False)
+        kind = r.choice(["none", "plain", "odd", "in place"])
+        res = out = None
+        if kind == "plain":
+            res = rnd(M, N, seed=s + 5)
+        elif kind == "odd":
+            res = rnd(M, N + 5, seed=s + 5)[:, 3:3 + N]
+        elif kind == "in place":
+            res = out = rnd(M, (N + 7) // 8 * 8 + 8, seed=s + 5)[:, :N]
+        keep = None if res is None else res.clone()
+        y = kb.linear(x, W, b, activation=act, residual=res, out=out, variant=r.choice(["auto", "auto_whole"]))
+        torch.cuda.synchronize()
+        check_linear(y, x, W, b, act, keep)
+    done()
+
+
 def test_linear_on_a_side_stream():
     x, W, b, r = linear_inputs(33, 1024, 1024, 70, True, True)
     want = kb.linear(x, W, b, residual=r)
@@ -284,6 +309,23 @@ def test_qk_norm_rope_many_rows(T, Hq, Hk):
     done()
     check_qk(yq, q, gq, table, pos, False)
     check_qk(yk, k, gk, table, pos, False)
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_qk_norm_rope_random_shapes(seed):
+    import random
+    r = random.Random(2000 + seed)
+    for i in range(30):
+        inter, D = r.random() < 0.5, 8 * r.randint(2, 32)
+        step = 8 if inter else 16
+        rot, T = step * r.randint(1, D // step), int(math.exp(r.uniform(0, math.log(9000))))
+        Hq, Hk = r.randint(1, 20), r.randint(1, 9)
+        q, k, gq, gk, pos = qk_inputs(T, Hq, Hk, D, 10 * i + seed, gamma=r.random() < 0.7)
+        table = kb.rope_table(4096, rot, device=DEV)
+        yq, yk = kb.qk_norm_rope(q, k, gq, gk, table, pos, interleaved=inter)
+        done()
+        check_qk(yq, q, gq, table, pos, inter)
+        check_qk(yk, k, gk, table, pos, inter)
 
 
 @pytest.mark.parametrize("inter", [False, True])
