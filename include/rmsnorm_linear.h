@@ -290,8 +290,8 @@ int rl_kv_cache_write_e4m3(const rl_kv_cache_write_args* args, void* stream);
  * v_out [total, H, D] is token i of sequence b, which lies in page page_table[b, i / page_size].
  *   page_table [B, max_pages] int32, leading dimension ld_pages; cu_seqlens [B + 1] int32, not decreasing, from 0.
  *   Rows from cu_seqlens[B] on are left as they are, or zeroed with zero_tail; tokens beyond `total` are not read.
- *   A page outside the cache, or a sequence longer than its table row: the row is left as it is and
- *   rl_take_device_status reports it.
+ *   A page outside the cache, or a sequence longer than its table row: the row is left as it is (with zero_tail zeroed)
+ *   and rl_take_device_status reports it.
  * Cache arguments and alignments as for rl_kv_cache_write_e4m3.  No workspace.  No reference counterpart. */
 typedef struct {
   rl_kv_cache_e4m3 cache;

@@ -814,6 +814,8 @@ inline bool mult8(std::initializer_list<int64_t> v) {
     if (x & 7) return false;
   return true;
 }
+// the stride of a dimension of one element (or none) says nothing
+inline int64_t stride_of(int64_t n, int64_t s) { return n > 1 ? s : 0; }
 inline bool fit_int(std::initializer_list<int64_t> v) {
   for (int64_t x : v)
     if (x < -0x7fffffffLL || x > 0x7fffffffLL) return false;
@@ -831,8 +833,10 @@ int check_cache(const rl_kv_cache_e4m3& a, KvCache* out) {
   if (!fit_int({a.num_pages, a.page_size, a.H, a.D}) || a.num_pages < 0 || a.page_size <= 0 || a.H <= 0 || a.D <= 0 || a.D > 256 ||
       !nonneg({a.code_page, a.code_token, a.code_head, a.scale_page, a.scale_token, a.scale_head}))
     return RL_ERR_BAD_SHAPE;
-  const KvCache c{(uint8_t*)a.k_codes, (uint8_t*)a.v_codes, a.k_scale, a.v_scale, a.code_page, a.code_token, a.code_head,
-                  a.scale_page, a.scale_token, a.scale_head, (int)a.num_pages, (int)a.page_size, (int)a.H, (int)a.D};
+  const KvCache c{(uint8_t*)a.k_codes, (uint8_t*)a.v_codes, a.k_scale, a.v_scale,
+                  stride_of(a.num_pages, a.code_page), stride_of(a.page_size, a.code_token), stride_of(a.H, a.code_head),
+                  stride_of(a.num_pages, a.scale_page), stride_of(a.page_size, a.scale_token), stride_of(a.H, a.scale_head),
+                  (int)a.num_pages, (int)a.page_size, (int)a.H, (int)a.D};
   const uintptr_t codes = reinterpret_cast<uintptr_t>(c.k_codes) | reinterpret_cast<uintptr_t>(c.v_codes);
   const uintptr_t scales = reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale);
   if ((codes & 7) || (scales & 3) || !mult8({c.D, c.c_page, c.c_off, c.c_head})) return RL_ERR_ALIGNMENT;
@@ -1168,10 +1172,12 @@ size_t rl_linear_workspace_bytes(int M, int N, int K) {
 
 int rl_linear_bf16(const rl_linear_args* args, void* stream) {
   if (!args) return RL_ERR_NULL_POINTER;
-  const auto [x, W, bias, residual, y, workspace, M64, N64, K64, ldx, ldw, ldr, ldy, activation, variant, ws_bytes] = *args;
+  const auto [x, W, bias, residual, y, workspace, M64, N64, K64, ldx_, ldw_, ldr_, ldy_, activation, variant, ws_bytes] = *args;
   if (!x || !W || !y) return RL_ERR_NULL_POINTER;
   if (!fit_int({M64, N64, K64}) || ws_bytes < 0) return RL_ERR_BAD_SHAPE;
   const int M = (int)M64, N = (int)N64, K = (int)K64;
+  // a single row's leading dimension says nothing
+  const int64_t ldx = M == 1 ? K : ldx_, ldw = N == 1 ? K : ldw_, ldr = M == 1 ? N : ldr_, ldy = M == 1 ? N : ldy_;
   const size_t workspace_bytes = (size_t)ws_bytes;
   if (M <= 0 || N <= 0 || K <= 0 || ldx < K || ldw < K || ldy < N || (residual && ldr != 0 && ldr < N))
     return RL_ERR_BAD_SHAPE;
@@ -1230,11 +1236,14 @@ int rl_linear_bf16(const rl_linear_args* args, void* stream) {
 int rl_qk_norm_rope_bf16(const rl_qk_norm_rope_args* args, void* stream) {
   if (!args) return RL_ERR_NULL_POINTER;
   const rl_qk_norm_rope_args& a = *args;
-  const auto [q, k, q_gamma, k_gamma, table, positions, q_out, k_out, T64, Hq64, Hk64, D64, rot64, n_positions64, ld_table, q_t, q_h,
-              k_t, k_h, qo_t, qo_h, ko_t, ko_h, positions_i64, interleaved, eps] = a;
+  const auto [q, k, q_gamma, k_gamma, table, positions, q_out, k_out, T64, Hq64, Hk64, D64, rot64, n_positions64, ld_table_, q_t_, q_h_,
+              k_t_, k_h_, qo_t_, qo_h_, ko_t_, ko_h_, positions_i64, interleaved, eps] = a;
   if (!q || !k || !table || !positions || !q_out || !k_out) return RL_ERR_NULL_POINTER;
   if (!fit_int({T64, Hq64, Hk64, D64, rot64, n_positions64})) return RL_ERR_BAD_SHAPE;
   const int T = (int)T64, Hq = (int)Hq64, Hk = (int)Hk64, D = (int)D64, rot = (int)rot64, n_positions = (int)n_positions64;
+  const int64_t q_t = stride_of(T, q_t_), q_h = stride_of(Hq, q_h_), k_t = stride_of(T, k_t_), k_h = stride_of(Hk, k_h_);
+  const int64_t qo_t = stride_of(T, qo_t_), qo_h = stride_of(Hq, qo_h_), ko_t = stride_of(T, ko_t_), ko_h = stride_of(Hk, ko_h_);
+  const int64_t ld_table = n_positions == 1 ? ((int64_t)rot + 3) / 4 * 4 : ld_table_;
   if (T <= 0 || Hq <= 0 || Hk <= 0 || D <= 0 || D > 256 || rot <= 0 || rot > D || n_positions < 0 || ld_table < rot ||
       (long long)Hq + Hk > 65536 || !nonneg({q_t, q_h, k_t, k_h, qo_t, qo_h, ko_t, ko_h}))
     return RL_ERR_BAD_SHAPE;
@@ -1280,13 +1289,14 @@ int rl_qk_norm_rope_bf16(const rl_qk_norm_rope_args* args, void* stream) {
 
 int rl_kv_cache_write_e4m3(const rl_kv_cache_write_args* args, void* stream) {
   if (!args) return RL_ERR_NULL_POINTER;
-  const auto [cache, k, v, slots, T64, k_t, k_h, v_t, v_h, slots_i64] = *args;
+  const auto [cache, k, v, slots, T64, k_t_, k_h_, v_t_, v_h_, slots_i64] = *args;
   if (!k || !v || !slots) return RL_ERR_NULL_POINTER;
   KvWriteParams p{};
   int rc = check_cache(cache, &p.c);
   if (rc) return rc;
   if (!fit_int({T64})) return RL_ERR_BAD_SHAPE;
   const int T = (int)T64, H = p.c.H, D = p.c.D;
+  const int64_t k_t = stride_of(T, k_t_), k_h = stride_of(H, k_h_), v_t = stride_of(T, v_t_), v_h = stride_of(H, v_h_);
   if (T <= 0 || H > 32768 || !nonneg({k_t, k_h, v_t, v_h})) return RL_ERR_BAD_SHAPE;
   if (!aligned16(k) || !aligned16(v) || !mult8({k_t, k_h, v_t, v_h}) ||
       (reinterpret_cast<uintptr_t>(slots) & (slots_i64 ? 7 : 3)))
@@ -1315,13 +1325,15 @@ int rl_kv_cache_write_e4m3(const rl_kv_cache_write_args* args, void* stream) {
 
 int rl_kv_cache_read_e4m3(const rl_kv_cache_read_args* args, void* stream) {
   if (!args) return RL_ERR_NULL_POINTER;
-  const auto [cache, page_table, cu_seqlens, k_out, v_out, total64, zero_tail, B64, max_pages64, ld_pages, ko_t, ko_h, vo_t, vo_h] = *args;
+  const auto [cache, page_table, cu_seqlens, k_out, v_out, total64, zero_tail, B64, max_pages64, ld_pages, ko_t_, ko_h_, vo_t_, vo_h_] =
+      *args;
   if (!k_out || !v_out || !cu_seqlens || (!page_table && B64 > 0 && max_pages64 > 0)) return RL_ERR_NULL_POINTER;
   KvReadParams p{};
   int rc = check_cache(cache, &p.c);
   if (rc) return rc;
   if (!fit_int({total64, B64, max_pages64})) return RL_ERR_BAD_SHAPE;
   const int total = (int)total64, B = (int)B64, max_pages = (int)max_pages64, H = p.c.H, D = p.c.D;
+  const int64_t ko_t = stride_of(total, ko_t_), ko_h = stride_of(H, ko_h_), vo_t = stride_of(total, vo_t_), vo_h = stride_of(H, vo_h_);
   if (total <= 0 || B < 0 || max_pages < 0 || ld_pages < 0 || H > 32768 || !nonneg({ko_t, ko_h, vo_t, vo_h})) return RL_ERR_BAD_SHAPE;
   if (!aligned16(k_out) || !aligned16(v_out) || !mult8({ko_t, ko_h, vo_t, vo_h}) ||
       ((reinterpret_cast<uintptr_t>(page_table) | reinterpret_cast<uintptr_t>(cu_seqlens)) & 3))

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_read_kernel(const KvReadPara
   const int lane = threadIdx.x & 31, c = lane & (G - 1);
   const int i = (int)(w / p.parts), part = (int)(w - (long long)i * p.parts);
   if (i >= p.T) return;
-  const bool held = p.B > 0 && i < p.cu[p.B];
+  bool held = p.B > 0 && i < p.cu[p.B];
   long long code_at = 0, scale_at = 0;
   if (!held) {
     if (!p.zero_tail) return;
@@ -175,11 +175,13 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_read_kernel(const KvReadPara
     const int page = (pos >= 0 && col < p.max_pages) ? p.pages[b * p.ld_pages + col] : -1;
     if (page < 0 || page >= p.c.num_pages) {
       if (lane == 0 && part == 0) record_bad_index(BAD_PAGE, i, page);
-      return;
+      if (!p.zero_tail) return;
+      held = false;  // (a fresh output: the row becomes zero)
+    } else {
+      const int off = pos - col * p.c.page_size;
+      code_at = page * p.c.c_page + off * p.c.c_off;
+      scale_at = page * p.c.s_page + off * p.c.s_off;
     }
-    const int off = pos - col * p.c.page_size;
-    code_at = page * p.c.c_page + off * p.c.c_off;
-    scale_at = page * p.c.s_page + off * p.c.s_off;
   }
   const int k_groups = (p.c.H + R - 1) / R;
   const int g0 = part * p.steps, g1 = min(g0 + p.steps, 2 * k_groups);

@@ -51,6 +51,8 @@ def _gamma_ok(g: torch.Tensor, D: int, dev: int) -> bool:
 
 
 _NEEDS = "heads of a multiple of 8 channels up to 256, strides of multiples of 8 elements, 16-byte aligned"
+_NEEDS_HALVES = _NEEDS + "; rotary_dim a multiple of 16 up to the head's"
+_NEEDS_NEIGHBOURS = _NEEDS + "; rotary_dim a multiple of 8 up to the head's"
 
 
 def _call(what: str, fn, args: bytes, dev: int, needs: str = _NEEDS) -> None:
@@ -122,22 +124,25 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: Optional[torch.Tenso
         q.data_ptr(), k.data_ptr(), 0 if q_gamma is None else q_gamma.data_ptr(), 0 if k_gamma is None else k_gamma.data_ptr(),
         table.data_ptr(), positions.data_ptr(), qo.data_ptr(), ko.data_ptr(), T, Hq, Hk, D, rot, P, table_strides[0], q_t, q_h,
         k_t, k_h, qo_t, qo_h, ko_t, ko_h, positions.dtype is torch.int64, interleaved, eps), dev,
-        f"{_NEEDS}; rotary_dim a multiple of {8 if interleaved else 16} up to the head's")
+        _NEEDS_NEIGHBOURS if interleaved else _NEEDS_HALVES)
     return qo, ko
 
 
 def _check_cache(k_codes, k_scale, v_codes, v_scale) -> Tuple[int, tuple]:
-    """The cache's device index, and its part of the C structures (without a copy of anything)."""
+    """The cache's device index, and its part of the C structures."""
+    if (isinstance(k_codes, torch.Tensor) and isinstance(k_scale, torch.Tensor) and isinstance(v_codes, torch.Tensor)
+            and isinstance(v_scale, torch.Tensor)):
+        dev, shape, c, scales, s = k_codes.get_device(), k_codes.shape, k_codes.stride(), k_scale.shape, k_scale.stride()
+        if (dev >= 0 and len(c) == 4 and c[3] == 1 and shape[:3] == scales and k_codes.dtype is _E4M3 and v_codes.dtype is _E4M3
+                and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and v_codes.get_device() == dev
+                and k_scale.get_device() == dev and v_scale.get_device() == dev and v_codes.shape == shape
+                and v_codes.stride() == c and v_scale.shape == scales and v_scale.stride() == s):
+            return dev, (k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *shape, c[0], c[1],
+                         c[2], *s)
     named = (("k_codes", k_codes), ("k_scale", k_scale), ("v_codes", v_codes), ("v_scale", v_scale))
     for name, t in named:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
-    dev, shape, c, s = k_codes.get_device(), k_codes.shape, k_codes.stride(), k_scale.stride()
-    if (dev >= 0 and len(c) == 4 and c[3] == 1 and len(s) == 3 and k_codes.dtype is _E4M3 and v_codes.dtype is _E4M3
-            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and v_codes.get_device() == dev
-            and k_scale.get_device() == dev and v_scale.get_device() == dev and v_codes.shape == shape
-            and v_codes.stride() == c and k_scale.shape == shape[:3] and v_scale.shape == shape[:3] and v_scale.stride() == s):
-        return dev, (k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *shape, c[0], c[1], c[2], *s)
     for name, t in named:
         dtype, nd = (_E4M3, 4) if name.endswith("codes") else (torch.float32, 3)
         if not t.is_cuda:
@@ -185,8 +190,8 @@ def kv_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.T
 
     `page_table` [B, max_pages] int32, `cu_seqlens` [B + 1] int32, not decreasing, from 0; both stay on the device, so
     `total` is the caller's: rows from cu_seqlens[B] on are zero in a fresh output and left as they are in `out`,
-    tokens beyond `total` are not read.  A page outside the cache (or a sequence longer than its table row) leaves the
-    row as it is, unspecified in a fresh output, and `check_status` raises."""
+    tokens beyond `total` are not read.  A row whose page lies outside the cache (or beyond its sequence's table row) is
+    left as it is, zero in a fresh output, and `check_status` raises."""
     dev, cache = _check_cache(k_codes, k_scale, v_codes, v_scale)
     H, D = cache[6], cache[7]
     strides = page_table.stride() if isinstance(page_table, torch.Tensor) else ()

@@ -154,6 +154,34 @@ def test_linear_extreme_values(act, M):
     assert bool(((y.double() - ref)[fine].abs() <= (HALF_STEP + 2.0 ** -14) * ref[fine].abs() + 1e-30).all())
 
 
+def test_single_rows_with_meaningless_strides():
+    """A dimension of one element may have any stride."""
+    K, N, D = 64, 72, 64
+    x = rnd(K, 1, seed=1).t()                                  # [1, K] with strides (1, 1)
+    W, r = rnd(N, K, seed=2), rnd(N, 1, seed=3).t()
+    y = kb.linear(x, W, residual=r)
+    w1 = kb.linear(rnd(5, K, seed=4), rnd(K, 1, seed=5).t())
+    done()
+    check_linear(y, x, W, None, None, r)
+    check_linear(w1, rnd(5, K, seed=4), rnd(K, 1, seed=5).t(), None, None, None)
+    q = rnd(2 * D + 7, seed=6)[:D].as_strided((1, 1, D), (3, 5, 1))
+    pos, table = torch.tensor([3], device=DEV), kb.rope_table(8, D, device=DEV)
+    yq, yk = kb.qk_norm_rope(q, q, None, None, table, pos)
+    one = kb.qk_norm_rope(q, q, None, None, table[3:4].as_strided((1, D), (1, 1)), pos - 3)
+    done()
+    check_qk(yq, q, None, table, pos, False)
+    assert torch.equal(yq, yk) and torch.equal(one[0], yq)
+    cache = [torch.zeros(D, dtype=torch.uint8, device=DEV).view(E4M3).as_strided((1, 1, 1, D), (5, 3, 1, 1)) if i % 2 == 0 else
+             torch.zeros(1, device=DEV).as_strided((1, 1, 1), (7, 7, 7)) for i in range(4)]
+    zero = torch.zeros(1, dtype=torch.int64, device=DEV)
+    kb.kv_cache_write(q, q, zero, *cache)
+    ko, vo = kb.kv_cache_read(*cache, torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([0, 1], dtype=torch.int32, device=DEV), 1)
+    done()
+    check_written(cache, q, q, zero)
+    val, sc = quant64(q)
+    assert torch.equal(ko.cpu(), (val.float() * sc[..., None]).to(BF16)) and torch.equal(ko, vo)
+
+
 def test_linear_refusals():
     x, W, b, r = linear_inputs(100, 64, 64, 1, True, True)
     for kw in (dict(activation="tanh"), dict(residual=r[:, :60]), dict(residual=r.float()), dict(out=x), dict(out=r[:, :32]),
@@ -614,9 +642,12 @@ def test_kv_cache_read_bad_pages_and_short_tables():
         for o, g in zip(out, good):
             assert torch.equal(o[:4], g[:4]) and bool((o[4:6] == 7.0).all()) and torch.equal(o[6:], g[6:])
     for cut in ([[0], [2]], [[], []]):            # sequences longer than their rows of the table
-        kb.kv_cache_read(*cache, torch.tensor(cut, dtype=torch.int32, device=DEV).view(2, -1), cu, 9)
+        fresh = kb.kv_cache_read(*cache, torch.tensor(cut, dtype=torch.int32, device=DEV).view(2, -1), cu, 9)
         with pytest.raises(RuntimeError, match="page"):
             kb.check_status()
+        for o, g in zip(fresh, good):             # a fresh output holds zeros there
+            n = 4 if cut[0] else 0
+            assert torch.equal(o[:n], g[:n]) and bool((o[n:6] == 0).all())
     for ends in ([5, 6, 9], [0, 9, 4], [-3, 2, 2 ** 31 - 1]):     # lengths that make no sense stay inside the table
         kb.kv_cache_read(*cache, torch.tensor([[0, 1], [2, -1]], dtype=torch.int32, device=DEV),
                          torch.tensor(ends, dtype=torch.int32, device=DEV), 9)

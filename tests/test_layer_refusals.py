@@ -166,6 +166,41 @@ def test_kv_cache_read_accepts(lib):
     assert passed(call_read(lib, vo=A[6] + 1024, kt=1024, vt=1024))    # keys and values of a token side by side
 
 
+@no_gpu
+def test_shared_memory_is_told_apart_from_interleaving(lib):
+    """Random strided outputs around each other: any shared byte is refused (never the other way round), and most
+    interleavings that share none are accepted."""
+    import itertools
+    import random
+    r = random.Random(5)
+    D, seen = 16, {True: 0, False: 0}
+    refused_apart = 0
+    for _ in range(4000):
+        T, Hq, Hk = r.randint(1, 4), r.randint(1, 4), r.randint(1, 4)
+        # strides of one parent array, heads or tokens outside, with gaps; the two outputs as windows of it, or as they come
+        if r.random() < 0.5:
+            inner = 16 * r.randint(1, 2)
+            outer = inner * r.randint(max(Hq, Hk), 10)
+            st = dict(qot=outer, qoh=inner, kot=outer, koh=inner)
+        else:
+            st = dict(qot=16 * r.randint(0, 8), qoh=16 * r.randint(0, 8), kot=16 * r.randint(0, 8), koh=16 * r.randint(0, 8))
+        shift = 16 * r.randint(-40, 40)
+
+        def covered(base, H, t, h):
+            return [base + a * t + b * h + d for a, b, d in itertools.product(range(T), range(H), range(0, D, 8))]
+
+        q, k = covered(0, Hq, st["qot"], st["qoh"]), covered(shift, Hk, st["kot"], st["koh"])
+        shares = len(set(q)) < len(q) or len(set(k)) < len(k) or bool(set(q) & set(k))
+        rc = call_qk(lib, qo=A[6], ko=A[6] + 2 * shift, T=T, Hq=Hq, Hk=Hk, D=D, rot=16, ldt=16, **st)
+        seen[shares] += 1
+        if shares:
+            assert rc == OVERLAP, (T, Hq, Hk, st, shift)
+        else:
+            refused_apart += rc == OVERLAP
+            assert rc == OVERLAP or passed(rc)
+    assert min(seen.values()) > 300 and refused_apart < 0.2 * seen[False]
+
+
 def test_argument_structures(lib):
     """The packed formats are the header's structures: pointers and 64-bit integers, no padding."""
     assert _lib.LINEAR_ARGS.size == 8 * 16 and _lib.QK_NORM_ROPE_ARGS.size == 8 * 26 and _lib.KV_CACHE_WRITE_ARGS.size == 8 * 23 and _lib.KV_CACHE_READ_ARGS.size == 8 * 27
