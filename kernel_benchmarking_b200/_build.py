@@ -11,7 +11,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.environ.get("RMSNORM_LINEAR_LIB") or os.path.join(PKG_DIR, "librmsnorm_linear.so")
 SOURCES = ["rl_api.cu"]
 HEADERS = ["rl_ptx.cuh", "rl_prefill.cuh", "rl_prefill_pair.cuh", "rl_decode.cuh", "rl_rowquant.cuh",
-           "rl_epilogue.cuh", "rl_rows.cuh", "rl_qk_rope.cuh", "rl_kv_cache.cuh"]
+           "rl_epilogue.cuh", "rl_linear_split.cuh", "rl_rows.cuh", "rl_qk_rope.cuh", "rl_kv_cache.cuh"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC", "-cudart", "static",

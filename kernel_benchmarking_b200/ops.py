@@ -306,10 +306,8 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
     if variant not in ("auto", "auto_whole"):
         raise ValueError(f"variant must be 'auto' or 'auto_whole', got {variant!r}")
     if out is None:
-        ldy = (N + 7) // 8 * 8
-        out = x.new_empty((M, ldy))
-        if ldy != N:
-            out = out[:, :N]
+        # rows of y start on 16-byte boundaries
+        out = x.new_empty((M, N)) if N % 8 == 0 else x.new_empty_strided((M, N), ((N + 7) // 8 * 8, 1))
     else:
         _check_out(out, M, N, x)
     if M == 0 or N == 0:
