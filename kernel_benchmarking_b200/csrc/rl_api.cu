@@ -539,11 +539,11 @@ struct SplitPlan {
 // microseconds.  Its figures are fits to measurements of 36 shapes with every tile and cluster size (tokens 1..4096, K
 // 256..14336): 5.5 us for a launch, its pipeline's start and its exchange (2 more for 128-token tiles, 0.25 per part), and
 // the k-blocks at 160 KB/us an SM with two CTAs or more on it, 85 with one.  The pairs: 10 us (8 without an epilogue, 12
-// with everything), and 0.34 per k-block of a round of tiles.  Measured, split against pairs: 128 x 4096 x 4096 13.6 / 20.4
-// us, 512 x 4096 x 4096 21.0 / 23.4, 1024^3 8.4 / 12.6, 1500 x 1536 x 1536 12.9 / 16.0, 4096 x 512 x 256 6.5 / 8.7; the
+// with everything), and 0.34 per k-block of a round of tiles.  Measured, split against pairs: 128 x 4096 x 4096 12.6 / 20.4
+// us, 512 x 4096 x 4096 20.7 / 23.4, 1024^3 8.0 / 12.6, 1500 x 1536 x 1536 12.7 / 16.0, 4096 x 512 x 256 6.6 / 8.7; the
 // other way round 512 x 4096 x 14336 58 / 53, 1024 x 4096 x 4096 34.7 / 29.9.  Up to 64 tokens it is always the former
-// (against the weight-streaming kernel of the norm: 16 x 4096 x 4096 9.9 / 13.2 us, 64 x 14336 x 4096 23.3 / 32, 64 x
-// 28672 x 4096 42.8 / 45.5).  The plan is arithmetic on the sizes, for the 148 SMs of a B200.
+// (against the weight-streaming kernel of the norm: 16 x 4096 x 4096 9.6 / 13.2 us, 64 x 14336 x 4096 23.4 / 32, 64 x
+// 28672 x 4096 41.4 / 45.5).  The plan is arithmetic on the sizes, for the 148 SMs of a B200.
 SplitPlan plan_split(int M, int N, int K) {
   constexpr int SMS = 148, PAIRS = 74;
   const int KB = (K + 63) / 64;

@@ -3,13 +3,15 @@
 //
 // Operands are swapped so that the 128-wide UMMA M dimension runs over output channels: A = W tile [128 x 64], B = x tile
 // [NT tokens x 64], D[channel, token] in tensor memory.  The `split` CTAs of a cluster (1, 2, 4 or 8) take one contiguous
-// part of the tile's k-blocks each, leave their fp32 accumulators in their own shared memory, and after one cluster barrier
-// each finishes its share of the tokens: it adds the parts in rank order out of its neighbours' shared memory, so results do
-// not depend on timing, and nothing is exchanged through global memory.  No workspace, no counters, and no CTA waits for
-// one outside its cluster, which the hardware schedules together.
+// part of the tile's k-blocks each.  Each then finishes a share of the tokens: once all have read their operands (a cluster
+// barrier that the read of tensor memory overlaps), every CTA stores its fp32 accumulators where the finishing ranks' operands
+// were, and after a second barrier each rank adds its tokens' parts in rank order out of its own shared memory.  Results do
+// not depend on timing, and nothing is exchanged through global memory: no workspace, no counters, and no CTA waits for one
+// outside its cluster, which the hardware schedules together.  (Parts left in place and read by the finishing ranks took
+// 3.4 us from the last MMA to the kernel's end on 333 x 1000 x 1144: the loads' round trips, and a barrier behind them.)
 //
 // Bound by W from HBM: 28672 x 4096 with 16 tokens in 39.9 us is 5920 GB/s, 90 % of the copy bandwidth; 4096 x 4096 (33 MB) in
-// 9.9 us is launch, first load and exchange as much as stream.  Ring depths and CTAs per SM: about 100 KB per CTA, two CTAs on
+// 9.6 us is launch, first load and exchange as much as stream.  Ring depths and CTAs per SM: about 100 KB per CTA, two CTAs on
 // an SM, so that one's start and exchange run under the other's stream.
 //
 // Warps: 0 TMA producer, 1 UMMA issuer, then the epilogue's.
@@ -48,11 +50,12 @@ struct SplitCfg {
 // where a wait that ran out is recorded (layout of the status block); part of the device image like g_index_status
 static __device__ int g_wait_status[RL_STATUS_INTS];
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
+// the two halves of cluster_sync_all
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // residual of tokens first and first + EW (zeros where there is none)
 template <int EW>
@@ -70,18 +73,16 @@ __device__ __forceinline__ void split_residual(const SplitParams& p, int m0, int
 // residual.  Two tokens at a time; `res` comes in with the first two's residual, and the next two's is on its way while
 // these are finished.
 template <int S, int EW>
-__device__ __forceinline__ void split_finish(const SplitParams& p, uint32_t part, int m0, int n, int first, int last,
-                                             const uint32_t (&bias)[2], uint2 (&res)[2]) {
-  uint32_t from[S];
-#pragma unroll
-  for (int r = 0; r < S; ++r) from[r] = mapa_shared(part, (uint32_t)r);
+__device__ __forceinline__ void split_finish(const SplitParams& p, const float4* part, int per, int m0, int n, int first,
+                                             int last, const uint32_t (&bias)[2], uint2 (&res)[2]) {
+  // part: this lane's four channels of [S][per][128] parts, the tokens first counted from the rank's first one (a multiple of per)
   for (int t0 = first; t0 < last; t0 += 2 * EW) {
     float4 v[2][S];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < S; ++r)
-        if (t0 + EW * u < last) v[u][r] = ld_cluster_f4(from[r] + (uint32_t)(t0 + EW * u) * 512u);
+        if (t0 + EW * u < last) v[u][r] = part[(r * per + ((t0 + EW * u) & (per - 1))) * 32];
     uint2 next[2];
     split_residual<EW>(p, m0, n, t0 + 2 * EW, last, next);
 #pragma unroll
@@ -133,6 +134,18 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   const int tt = tile % p.token_tiles, ct = tile / p.token_tiles;
   const int KB = (p.K + 63) >> 6;
   const int kb0 = (int)((long long)rank * KB / S), kb1 = (int)((long long)(rank + 1) * KB / S);  // never empty: S <= KB
+  const int m0 = tt * NT, n0 = ct * 128;
+  const int tokens = min(NT, p.M - m0);
+  const int n_pre = min(STAGES, kb1 - kb0);  // k-blocks whose loads go out before the CTA-wide sync
+
+  // W is read once where one tile holds all tokens; x, and W otherwise, by several clusters
+  const bool w_once = p.token_tiles == 1;
+  auto issue = [&](int s, int kb, uint64_t pol_w, uint64_t pol_x) {
+    mbar_expect_tx(bar_full(s), Cfg::W_BYTES + Cfg::X_BYTES);
+    if (w_once) tma_load_2d_hint(sbase + Cfg::OFF_W + s * Cfg::W_BYTES, &tm_w, bar_full(s), kb * 64, n0, pol_w);
+    else tma_load_2d(sbase + Cfg::OFF_W + s * Cfg::W_BYTES, &tm_w, bar_full(s), kb * 64, n0);
+    tma_load_2d_hint(sbase + Cfg::OFF_X + s * Cfg::X_BYTES, &tm_x, bar_full(s), kb * 64, m0, pol_x);
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -146,6 +159,10 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     fence_mbar_init();
     prefetch_tmap(&tm_w);
     prefetch_tmap(&tm_x);
+    grid_dependency_wait();
+    // fill the ring right away: the first loads need neither tensor memory nor the other warps
+    const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
+    for (int i = 0; i < n_pre; ++i) issue(i, kb0 + i, pol_w, pol_x);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
@@ -159,8 +176,6 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   launch_dependents();
   grid_dependency_wait();
 
-  const int m0 = tt * NT, n0 = ct * 128;
-  const int tokens = min(NT, p.M - m0);
   // the tokens this warp will finish (rank's share, from `first` in steps of EW), and what that needs early: the bias of the
   // lane's four channels and the first tokens' residual
   const int per = NT / S;
@@ -175,19 +190,12 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   }
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    // W is read once where one tile holds all tokens; x, and W otherwise, by several clusters
     const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
-    const bool w_once = p.token_tiles == 1;
     int s = 0;
-    uint32_t ph = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    uint32_t ph = 1;  // (the first turn of the ring is on its way already)
+    for (int kb = kb0 + STAGES; kb < kb1; ++kb) {
       if (!mbar_wait_warp(bar_empty(s), ph ^ 1, ctl, 0, STAGES + s, kb)) break;
-      if (elect_one()) {
-        mbar_expect_tx(bar_full(s), Cfg::W_BYTES + Cfg::X_BYTES);
-        if (w_once) tma_load_2d_hint(sbase + Cfg::OFF_W + s * Cfg::W_BYTES, &tm_w, bar_full(s), kb * 64, n0, pol_w);
-        else tma_load_2d(sbase + Cfg::OFF_W + s * Cfg::W_BYTES, &tm_w, bar_full(s), kb * 64, n0);
-        tma_load_2d_hint(sbase + Cfg::OFF_X + s * Cfg::X_BYTES, &tm_x, bar_full(s), kb * 64, m0, pol_x);
-      }
+      if (elect_one()) issue(s, kb, pol_w, pol_x);
       __syncwarp();
       if (++s == STAGES) { s = 0; ph ^= 1; }
     }
@@ -213,45 +221,56 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     if (ok && elect_one()) umma_commit(bar_acc);
     __syncwarp();
   } else {
-    // ------------------------------------------------------------ accumulator -> own shared memory, [token][channel]
-    const int q = warp & 3;
-    if (mbar_wait_warp(bar_acc, 0, ctl, 2, 2 * STAGES, kb0)) {
-      tc_fence_after();
-      float* part = reinterpret_cast<float*>(smem);  // every operand has been read
-      const int ch = q * 32 + lane;
-      constexpr int HALVES = EW / 4;  // a quarter's two warps share the tokens
-      const int half = (warp - 2) >> 2;
-#pragma unroll
-      for (int hh = 0; hh < NT / 16 / HALVES; ++hh) {
-        const int h = hh * HALVES + half;
-        if (h * 16 >= tokens) break;
-        uint32_t v[16];
-        tmem_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + h * 16, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) part[(h * 16 + j) * 128 + ch] = __uint_as_float(v[j]);
-      }
-      tc_fence_before();
-    }
+    mbar_wait_warp(bar_acc, 0, ctl, 2, 2 * STAGES, kb0);
   }
-  __syncthreads();
-  const int my_abort = ctl->abort;
+  // ------------------------------------------------------------ accumulators -> the finishing ranks, [S][per][128 channels]
+  // This CTA's MMAs are done (or a wait of it ran out, which it has recorded; the barriers are reached all the same).
+  if (S > 1) cluster_arrive();
+  tc_fence_after();
+  const int q = warp & 3, half = (warp - 2) >> 2;
+  constexpr int HALVES = EW / 4;  // a quarter's two warps share the tokens
+  uint32_t v[16];
+  auto load16 = [&](int h) {
+    tmem_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + h * 16, v);
+    tmem_wait_ld();
+  };
+  const bool mine = warp >= 2 && half * 16 < tokens;
+  if (mine) load16(half);
+  if (S > 1) cluster_wait();  // every rank's operands have been read: their place may be written
+  else __syncthreads();
+  if (mine) {
+    const int per_log2 = 31 - __clz(per);  // NT and S are powers of two
+    const uint32_t to = sbase + (uint32_t)(rank * per * 128 + q * 32 + lane) * 4u;
+#pragma unroll
+    for (int hh = 0; hh < NT / 16 / HALVES; ++hh) {
+      const int h = hh * HALVES + half;
+      if (h * 16 >= tokens) break;
+      if (hh > 0) load16(h);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int tk = h * 16 + j, r = tk >> per_log2;
+        if (tk < tokens) st_cluster_f32(mapa_shared(to + (uint32_t)(tk - r * per) * 512u, (uint32_t)r), __uint_as_float(v[j]));
+      }
+    }
+    tc_fence_before();
+  }
   if (S > 1) cluster_sync_all();
+  else __syncthreads();
+  const int my_abort = ctl->abort;
   if (warp >= 2 && !my_abort) {
     // ------------------------------------------------------------ this rank's tokens
-    const uint32_t part = sbase + lane * 16u;
-    if (S == 1) split_finish<1, EW>(p, part, m0, n0 + lane * 4, first, last, bias, res);
-    else if (S == 2) split_finish<2, EW>(p, part, m0, n0 + lane * 4, first, last, bias, res);
-    else if (S == 4) split_finish<4, EW>(p, part, m0, n0 + lane * 4, first, last, bias, res);
-    else split_finish<8, EW>(p, part, m0, n0 + lane * 4, first, last, bias, res);
+    const float4* part = reinterpret_cast<const float4*>(smem) + lane;
+    if (S == 1) split_finish<1, EW>(p, part, per, m0, n0 + lane * 4, first, last, bias, res);
+    else if (S == 2) split_finish<2, EW>(p, part, per, m0, n0 + lane * 4, first, last, bias, res);
+    else if (S == 4) split_finish<4, EW>(p, part, per, m0, n0 + lane * 4, first, last, bias, res);
+    else split_finish<8, EW>(p, part, per, m0, n0 + lane * 4, first, last, bias, res);
   }
   // ------------------------------------------------------------ teardown
   if (my_abort) {  // copies still in flight must land before the shared memory is given up
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
-  __syncthreads();
-  if (S > 1) cluster_sync_all();  // nobody leaves while a neighbour may still read its part
+  // (nobody touches a neighbour's shared memory after the second barrier)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, Cfg::TMEM_COLS);

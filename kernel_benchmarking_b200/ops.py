@@ -252,11 +252,13 @@ def _linear_workspace_bytes(M: int, N: int, K: int) -> int:
     return _lib.load().rl_linear_workspace_bytes(M, N, K)
 
 
-def _matrix_ok(t: torch.Tensor, dev: int) -> bool:
-    if not isinstance(t, torch.Tensor):
-        return False
-    strides = t.stride()
-    return t.dtype is torch.bfloat16 and t.get_device() == dev and len(strides) == 2 and strides[1] == 1
+def _explain_linear(x, W, residual) -> None:
+    """What `linear` expects of its matrices, in the words of whichever is wrong."""
+    _check_matrix("x", x, torch.bfloat16)
+    _check_matrix("W", W, torch.bfloat16)
+    if residual is not None:
+        _check_matrix("residual", residual, torch.bfloat16)
+    raise ValueError("x, W and residual must be on one device")
 
 
 def linear_workspace(M: int, N: int, K: int, device: Optional[torch.device] = None) -> torch.Tensor:
@@ -284,13 +286,18 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
     captured into a CUDA graph takes a workspace of its own from the graph's memory and clears it on every replay, so
     graphs share none; a `linear_workspace` passed in saves that step."""
     # one plain condition on the path of every decode step; what is wrong is looked for only when it fails
-    dev = x.get_device() if isinstance(x, torch.Tensor) else -1
-    if dev < 0 or not (_matrix_ok(x, dev) and _matrix_ok(W, dev) and (residual is None or _matrix_ok(residual, dev))):
-        _check_matrix("x", x, torch.bfloat16)
-        _check_matrix("W", W, torch.bfloat16)
-        if residual is not None:
-            _check_matrix("residual", residual, torch.bfloat16)
-        raise ValueError("x, W and residual must be on one device")
+    if not isinstance(x, torch.Tensor) or not isinstance(W, torch.Tensor):
+        _explain_linear(x, W, residual)
+    dev, xs, ws_ = x.get_device(), x.stride(), W.stride()
+    if (dev < 0 or x.dtype is not torch.bfloat16 or W.dtype is not torch.bfloat16 or W.get_device() != dev or len(xs) != 2
+            or xs[1] != 1 or len(ws_) != 2 or ws_[1] != 1):
+        _explain_linear(x, W, residual)
+    ldr = 0
+    if residual is not None:
+        rs = residual.stride() if isinstance(residual, torch.Tensor) else ()
+        if len(rs) != 2 or rs[1] != 1 or residual.dtype is not torch.bfloat16 or residual.get_device() != dev:
+            _explain_linear(x, W, residual)
+        ldr = rs[0]
     M, K = x.shape
     N, K2 = W.shape
     if K2 != K:
@@ -317,34 +324,33 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
                                       and workspace.dtype is torch.uint8 and workspace.is_contiguous()
                                       and workspace.numel() >= nbytes):
         raise ValueError(f"workspace must be at least {nbytes} contiguous bytes on x's device (linear_workspace)")
+    args = (x.data_ptr(), W.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
+            out.data_ptr())
+    sizes = (M, N, K, xs[0], ws_[0], ldr, out.stride()[0], act, _lib.VARIANTS[variant])
     if dev == torch.cuda.current_device():
-        rc = _launch_linear(dev, x, W, bias, residual, out, M, N, K, act, workspace, nbytes, variant)
+        rc = _launch_linear(dev, args, sizes, workspace, nbytes)
     else:
         with torch.cuda.device(dev):
-            rc = _launch_linear(dev, x, W, bias, residual, out, M, N, K, act, workspace, nbytes, variant)
+            rc = _launch_linear(dev, args, sizes, workspace, nbytes)
     if rc:
         _lib.check(rc, "rl_linear_bf16")
     return out
 
 
-def _launch_linear(dev, x, W, bias, residual, out, M, N, K, act, ws, nbytes, variant) -> int:
+def _launch_linear(dev: int, pointers: tuple, sizes: tuple, ws: Optional[torch.Tensor], nbytes: int) -> int:
     lib = _lib.load()
     stream = _raw_stream(dev)
     if nbytes == 0:
-        ws_ptr = ws_bytes = 0
         _status_devices.add(dev)
-    elif ws is None:
+        return lib.rl_linear_bf16(_lib.LINEAR_ARGS.pack(*pointers, 0, *sizes, 0), stream)
+    if ws is None:
+        device = torch.device("cuda", dev)
         if torch.cuda.is_current_stream_capturing():
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _lib.check(lib.rl_workspace_init(ws.data_ptr(), _CLEAN_BYTES, stream), "rl_workspace_init")
         else:
-            ws = _workspace(x.device, nbytes, stream)
-    if nbytes:
-        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
-    return lib.rl_linear_bf16(_lib.LINEAR_ARGS.pack(
-        x.data_ptr(), W.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
-        out.data_ptr(), ws_ptr, M, N, K, x.stride(0), W.stride(0), 0 if residual is None else residual.stride(0), out.stride(0),
-        act, _lib.VARIANTS[variant], ws_bytes), stream)
+            ws = _workspace(device, nbytes, stream)
+    return lib.rl_linear_bf16(_lib.LINEAR_ARGS.pack(*pointers, ws.data_ptr(), *sizes, ws.numel()), stream)
 
 
 def quantize_rows_e4m3(x: torch.Tensor, gamma: Optional[torch.Tensor], eps: float = 1e-6):
