@@ -772,7 +772,7 @@ bool disjoint(const View& a, const View& b, int i = 0, int j = 0, int64_t shift 
 // How the rows of `tokens` tokens are dealt to warps: every token has `groups` groups of 32 / G rows, a warp takes `steps`
 // of them.  As many as leave 24 warps for every SM - each then has several loads in flight and makes what it needs per
 // token once -, one where there are few rows and only latency counts.  Measured at 16384 tokens and more, all of a token's
-// groups in one warp against half of them: norm and rotation of 10 groups 60.5 / 78 us, write of 4 groups 20.9 / 23.3, read
+// groups in one warp against half of them: norm and rotation of 10 groups 60.5 / 78 us, write of 4 groups 20.3 / 23.3, read
 // of 4 groups 126 / 141.
 inline int lanes_per_row(int D) {
   int g = 1;

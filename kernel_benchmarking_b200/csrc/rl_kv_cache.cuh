@@ -6,7 +6,7 @@
 // NaN and does not count for a; a row with an infinity reads back as NaN throughout.
 //
 // Both kernels move bytes: 3 D + 4 per row, read and written together.  131072 tokens of 8 heads of 128 are read back in 126
-// us (6460 GB/s, 99 % of the copy bandwidth); 16384 are written in 20.9 us (4860 GB/s), of which 2 are the launch: the
+// us (6460 GB/s, 99 % of the copy bandwidth); 16384 are written in 20.3 us (5010 GB/s), of which 2 are the launch: the
 // reduction, the two divisions and the exact rounding keep the SMs issuing for two thirds of the time.
 #pragma once
 #include <cuda_fp8.h>
@@ -63,22 +63,25 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_write_kernel(const KvWritePa
   const int k_groups = (p.c.H + R - 1) / R;  // the key heads' groups, then as many of the value heads
   const int g0 = part * p.steps, g1 = min(g0 + p.steps, 2 * k_groups);
   uint32_t x[U][2][4];
-  auto load_rows = [&](int g) {
+  // U groups from g, all of one kind (below `end`)
+  auto load_rows = [&](int g, int end) {
+    const bool is_k = g < k_groups;
+    const __nv_bfloat16* src = (is_k ? p.k + (size_t)t * p.k_t : p.v + (size_t)t * p.v_t) + c * 8;
+    const long long src_h = is_k ? p.k_h : p.v_h;
+    const int h0 = (is_k ? g : g - k_groups) * R + lane / G;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool is_k = g + u < k_groups;
-      const int h = (is_k ? g + u : g + u - k_groups) * R + lane / G;
-      const __nv_bfloat16* src = is_k ? p.k + (size_t)t * p.k_t + h * p.k_h : p.v + (size_t)t * p.v_t + h * p.v_h;
+      const int h = h0 + u * R;
+      const bool row = g + u < end && h < p.c.H;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int ch = c + j * G;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (g + u < g1 && h < p.c.H && ch * 8 < p.c.D) v = *reinterpret_cast<const uint4*>(src + ch * 8);
+        if (row && (c + j * G) * 8 < p.c.D) v = *reinterpret_cast<const uint4*>(src + h * src_h + j * G * 8);
         x[u][j][0] = v.x; x[u][j][1] = v.y; x[u][j][2] = v.z; x[u][j][3] = v.w;
       }
     }
   };
-  load_rows(g0);  // on their way while the slot is looked up
+  load_rows(g0, g0 < k_groups ? min(g1, k_groups) : g1);  // on their way while the slot is looked up
   const long long slot = load_index(p.slots, t, p.slots64);
   if (slot < 0) return;
   const long long page = slot / p.c.page_size;
@@ -87,14 +90,18 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_write_kernel(const KvWritePa
     if (lane == 0 && part == 0) record_bad_index(BAD_SLOT, t, slot);
     return;
   }
-  const long long code_at = page * p.c.c_page + off * p.c.c_off, scale_at = page * p.c.s_page + off * p.c.s_off;
+  const long long code_at = page * p.c.c_page + off * p.c.c_off + c * 8, scale_at = page * p.c.s_page + off * p.c.s_off;
 #pragma unroll 1
-  for (int g = g0; g < g1; g += U) {
-    if (g > g0) load_rows(g);
+  for (int g = g0; g < g1;) {
+    const bool is_k = g < k_groups;
+    const int end = is_k ? min(g1, k_groups) : g1;
+    if (g > g0) load_rows(g, end);
+    uint8_t* codes = (is_k ? p.c.k_codes : p.c.v_codes) + code_at;
+    float* scales = (is_k ? p.c.k_scale : p.c.v_scale) + scale_at;
+    const int h0 = (is_k ? g : g - k_groups) * R + lane / G;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool is_k = g + u < k_groups;
-      const int h = (is_k ? g + u : g + u - k_groups) * R + lane / G;
+      const int h = h0 + u * R;
       // largest |x| of the row, NaN left out
       __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
@@ -110,16 +117,15 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_write_kernel(const KvWritePa
       }
       const float a = fmaxf(fmaxf(bf16lo(mu), bf16hi(mu)), 0x1p-100f);
       const float inv = 448.0f / a;
-      if (g + u < g1 && h < p.c.H) {
-        uint8_t* dst = (is_k ? p.c.k_codes : p.c.v_codes) + code_at + h * p.c.c_head;
+      if (g + u < end && h < p.c.H) {
+        uint8_t* dst = codes + h * p.c.c_head;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int ch = c + j * G;
-          if (ch * 8 < p.c.D) *reinterpret_cast<uint2*>(dst + ch * 8) = e4m3_codes(x[u][j], inv);
-        }
-        if (c == 0) (is_k ? p.c.k_scale : p.c.v_scale)[scale_at + h * p.c.s_head] = a / 448.0f;
+        for (int j = 0; j < 2; ++j)
+          if ((c + j * G) * 8 < p.c.D) *reinterpret_cast<uint2*>(dst + j * G * 8) = e4m3_codes(x[u][j], inv);
+        if (c == 0) scales[h * p.c.s_head] = a / 448.0f;
       }
     }
+    g = (g + U < end) ? g + U : end;
   }
 }
 
