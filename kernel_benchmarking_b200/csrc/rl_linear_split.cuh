@@ -69,13 +69,13 @@ __device__ __forceinline__ void split_residual(const SplitParams& p, int m0, int
   }
 }
 
-// The tokens first, first + EW, .. below `last` of a tile (EW epilogue warps), four channels per lane: parts in rank order, bias, activation,
-// residual.  Two tokens at a time; `res` comes in with the first two's residual, and the next two's is on its way while
-// these are finished.
+// The tokens first, first + EW, .. below `last` of a tile (EW epilogue warps), four channels per lane: parts in rank order,
+// bias, activation, residual.  `part` is this lane's place in the rank's [S][per][128] parts, whose tokens count from a
+// multiple of per.  Two tokens at a time; `res` comes in with the first two's residual, and the next two's is on its way
+// while these are finished.
 template <int S, int EW>
 __device__ __forceinline__ void split_finish(const SplitParams& p, const float4* part, int per, int m0, int n, int first,
                                              int last, const uint32_t (&bias)[2], uint2 (&res)[2]) {
-  // part: this lane's four channels of [S][per][128] parts, the tokens first counted from the rank's first one (a multiple of per)
   for (int t0 = first; t0 < last; t0 += 2 * EW) {
     float4 v[2][S];
 #pragma unroll

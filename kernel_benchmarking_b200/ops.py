@@ -278,6 +278,7 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
     """activation(x [M, K] @ W [N, K].t() + bias [N]) + residual [M, N], all bf16, in one kernel: fp32 from the product to
     the one rounding of the result.  The projection behind an attention or an MLP, added to the residual stream.
 
+    K a multiple of 8, rows and vectors 16-byte aligned; with more than 64 tokens that goes for the rows of `out` as well.
     `activation`: None, "relu", "gelu" (erf), "gelu_tanh" or "silu".  `residual` may be `out` itself (an update in
     place), or one row expanded to all tokens; `out` may share no other memory with the inputs.
 

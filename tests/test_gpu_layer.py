@@ -12,10 +12,8 @@ import math
 
 import pytest
 import torch
-import torch.nn.functional as F
 
 import kernel_benchmarking_b200 as kb
-from kernel_benchmarking_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -95,6 +93,27 @@ def test_linear_large(M, N, K, act, bias, residual):
     check_linear(y, x, W, b, act, r)
     check_linear(whole, x, W, b, act, r)
     assert torch.equal(y, again)
+
+
+@pytest.mark.parametrize("M,N,K,act,bias,residual", [
+    (8192, 4096, 13312, "gelu", True, True),         # 256 tiles of 256 x 512: the last 34 cut in two
+    (5800, 5000, 13320, "gelu_tanh", True, True),    # 230, ragged: the last 8 cut in four
+    (5800, 5000, 8200, None, False, True),
+    (5800, 5000, 9224, "silu", False, False)])
+def test_linear_on_wide_tiles(M, N, K, act, bias, residual):
+    """K-loops long enough for the 256 x 512 tiles' exposed epilogue, whole and with a last round cut along K; in place."""
+    x, W, b, r = linear_inputs(M, N, K, 15, bias, residual)
+    whole = kb.linear(x, W, b, activation=act, residual=r, variant="auto_whole")
+    y = kb.linear(x, W, b, activation=act, residual=r)
+    again = kb.linear(x, W, b, activation=act, residual=r)
+    done()
+    check_linear(y, x, W, b, act, r)
+    check_linear(whole, x, W, b, act, r)
+    assert torch.equal(y, again)
+    if r is not None:
+        kb.linear(x, W, b, activation=act, residual=r, out=r)
+        done()
+        assert torch.equal(r, y)
 
 
 @pytest.mark.parametrize("M,N,K,pairs", [(300, 520, 328, False), (2048, 5120, 2048, True), (8192, 7168, 4096, True)])
