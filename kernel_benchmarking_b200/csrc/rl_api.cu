@@ -537,12 +537,14 @@ struct SplitPlan {
 };
 // Cluster-split kernel or CTA pairs, and the former's tile and cluster size: the least of what a short model says, in
 // microseconds.  Its figures are fits to measurements of 36 shapes with every tile and cluster size (tokens 1..4096, K
-// 256..14336): 5.5 us for a launch, its pipeline's start and its exchange (2 more for 128-token tiles, 0.25 per part), and
-// the k-blocks at 160 KB/us an SM with two CTAs or more on it, 85 with one.  The pairs: 10 us (8 without an epilogue, 12
+// 256..14336): 4.5 us for a launch, its pipeline's start and its exchange, 5.9 where SMs take a second CTA, which starts a
+// microsecond later (1 more for 128-token tiles, 0.05 per part, 0.012 per token that a CTA finishes), and the k-blocks at
+// 160 KB/us an SM with two CTAs on it, 100 with one.  So 64 x 4096 x 4096 runs in 128 CTAs (10.7 us) rather than 256 (12.0), 333 x 1000 x 1144 in 96 (6.8)
+// rather than 192 (8.0), 128 x 4096 x 4096 in 256 (12.7) rather than 128 (14.0).  The pairs: 10 us (8 without an epilogue, 12
 // with everything), and 0.34 per k-block of a round of tiles.  Measured, split against pairs: 128 x 4096 x 4096 12.6 / 20.4
 // us, 512 x 4096 x 4096 20.7 / 23.4, 1024^3 8.0 / 12.6, 1500 x 1536 x 1536 12.7 / 16.0, 4096 x 512 x 256 6.6 / 8.7; the
 // other way round 512 x 4096 x 14336 58 / 53, 1024 x 4096 x 4096 34.7 / 29.9.  Up to 64 tokens it is always the former
-// (against the weight-streaming kernel of the norm: 16 x 4096 x 4096 9.6 / 13.2 us, 64 x 14336 x 4096 23.4 / 32, 64 x
+// (against the weight-streaming kernel of the norm: 16 x 4096 x 4096 9.0 / 13.2 us, 64 x 14336 x 4096 23.4 / 32, 64 x
 // 28672 x 4096 41.4 / 45.5).  The plan is arithmetic on the sizes, for the 148 SMs of a B200.
 SplitPlan plan_split(int M, int N, int K) {
   constexpr int SMS = 148, PAIRS = 74;
@@ -555,8 +557,9 @@ SplitPlan plan_split(int M, int N, int K) {
     for (int s = 1; s <= 8 && (s == 1 || (tiles * s <= 2 * SMS && KB >= 2 * s)); s *= 2) {
       const long long ctas = tiles * s, per_sm = (ctas + SMS - 1) / SMS;
       if (M > 64 && per_sm > 2) break;
-      const double kb_us = (16.0 + nt / 8.0) / (per_sm >= 2 ? 160.0 : 85.0);
-      const double us = 5.5 + (double)per_sm * ((KB + s - 1) / s) * kb_us + 0.25 * s + (nt == 128 ? 2.0 : 0.0);
+      const double kb_us = (16.0 + nt / 8.0) / (per_sm >= 2 ? 160.0 : 100.0);
+      const double us = (per_sm >= 2 ? 5.9 : 4.5) + (double)per_sm * ((KB + s - 1) / s) * kb_us + 0.05 * s + 0.012 * nt / s +
+                        (nt == 128 ? 1.0 : 0.0);
       if (us < best_us) { best_us = us; best = SplitPlan{nt, s}; }
     }
   }

@@ -11,7 +11,7 @@
 // 3.4 us from the last MMA to the kernel's end on 333 x 1000 x 1144: the loads' round trips, and a barrier behind them.)
 //
 // Bound by W from HBM: 28672 x 4096 with 16 tokens in 39.9 us is 5920 GB/s, 90 % of the copy bandwidth; 4096 x 4096 (33 MB) in
-// 9.6 us is launch, first load and exchange as much as stream.  Ring depths and CTAs per SM: about 100 KB per CTA, two CTAs on
+// 9.0 us is launch, first load and exchange as much as stream.  Ring depths and CTAs per SM: about 100 KB per CTA, two CTAs on
 // an SM, so that one's start and exchange run under the other's stream.
 //
 // Warps: 0 TMA producer, 1 UMMA issuer, then the epilogue's.
