@@ -226,8 +226,9 @@ int rl_lora_linear_bf16(const void* a, const void* b, const void* xa, const void
  *   Few tokens or few tiles run a kernel that shares every tile's k-loop among the CTAs of a cluster and needs no
  *   workspace (rl_linear_workspace_bytes is 0; a wait that ran out is reported by rl_take_device_status); the others run
  *   the CTA-pair tiles.
- *   workspace: rl_linear_workspace_bytes(M, N, K) bytes, as for every operator here zeroed once, one per stream (one that
- *   ends before the k-split blocks is accepted; every tile is then computed whole).
+ *   workspace: rl_linear_workspace_bytes(M, N, K) bytes, 16-byte aligned and apart from the operands, as for every operator
+ *   here zeroed once, one per stream (one that ends before the k-split blocks is accepted; every tile is then computed
+ *   whole).
  *   variant: RL_VARIANT_AUTO or RL_VARIANT_AUTO_WHOLE (see Concurrency above).
  * No reference counterpart beyond its plain GEMM (demo/new_profiling/rmsnorm_linear_new.py:29-31). */
 size_t rl_linear_workspace_bytes(int M, int N, int K);

@@ -1201,6 +1201,13 @@ int rl_linear_bf16(const rl_linear_args* args, void* stream) {
   const SplitPlan plan = plan_split(M, N, K);
   const WsLayout wl = ws_layout(M, N);
   if (plan.nt == 0 && (!workspace || workspace_bytes < wl.min_total)) return RL_ERR_WORKSPACE;
+  if (plan.nt == 0) {
+    if (!aligned16(workspace)) return RL_ERR_ALIGNMENT;  // the parts of cut tiles are stored 16 bytes at a time
+    const View vw(workspace, 1, {{(int64_t)std::min(workspace_bytes, wl.tail_total), 1}});
+    if (!disjoint(vw, vy) || !disjoint(vw, View(x, 2, {{M, ldx}, {K, 1}})) || !disjoint(vw, View(W, 2, {{N, ldw}, {K, 1}})) ||
+        (bias && !disjoint(vw, View(bias, 2, {{N, 1}}))) || (residual && !disjoint(vw, View(residual, 2, {{M, ldr}, {N, 1}}))))
+      return RL_ERR_OVERLAP;
+  }
   DeviceInfo di;
   int rc = device_info(&di);
   if (rc) return rc;

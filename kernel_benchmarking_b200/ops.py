@@ -285,7 +285,7 @@ def linear(x: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor] = None
     Few tokens or few tiles need no scratch.  The others use one workspace per device and stream, as the other operators
     do, and `variant="auto_whole"` belongs on streams that run concurrently (see `rmsnorm_linear`).  A call that is being
     captured into a CUDA graph takes a workspace of its own from the graph's memory and clears it on every replay, so
-    graphs share none; a `linear_workspace` passed in saves that step."""
+    graphs share none; a `linear_workspace` passed in saves that step (16-byte aligned, apart from the operands)."""
     # one plain condition on the path of every decode step; what is wrong is looked for only when it fails
     if not isinstance(x, torch.Tensor) or not isinstance(W, torch.Tensor):
         _explain_linear(x, W, residual)

@@ -220,6 +220,24 @@ def test_linear_refusals():
     done()
 
 
+def test_linear_workspaces_that_start_anywhere():
+    """A slice of a larger buffer serves from any 16-byte boundary; elsewhere, and inside an operand, it is refused."""
+    M, N, K = 4096, 1536, 4096   # cuts tiles along K
+    x, W, b, r = linear_inputs(M, N, K, 61, True, True)
+    want = kb.linear(x, W, b, residual=r)
+    n = kb.linear_workspace(M, N, K, x.device).numel()
+    assert n > 0
+    flat = torch.zeros(n + 64, dtype=torch.uint8, device=DEV)
+    for at in (4, 8, 17):
+        with pytest.raises(ValueError, match="aligned"):
+            kb.linear(x, W, b, residual=r, workspace=flat[at:])
+    assert torch.equal(kb.linear(x, W, b, residual=r, workspace=flat[16:]), want)
+    big = torch.zeros(n // 2 + M * N, dtype=BF16, device=DEV)
+    with pytest.raises(ValueError, match="shares memory"):
+        kb.linear(x, W, b, workspace=big.view(torch.uint8), out=big[:M * N].view(M, N))
+    done()
+
+
 @pytest.mark.parametrize("M,N,K", [(8, 2048, 1024), (300, 520, 1024), (4096, 2048, 4096)])
 @pytest.mark.parametrize("own", [False, True])
 def test_linear_in_two_graphs_at_once(M, N, K, own):

@@ -53,6 +53,24 @@ def test_linear_refuses(lib, rc, kw):
     assert call_linear(lib, **kw) == rc
 
 
+# (made-up matrices of 4096 x 4096, 32 MiB each, a gigabyte and more apart)
+BIG = dict(M=4096, N=4096, K=4096, ldx=4096, ldw=4096, ldr=4096, ldy=4096, **FAR)
+
+
+@pytest.mark.parametrize("rc,ws", [(ALIGN, 0x10000000004), (ALIGN, 0x10000000008), (OVERLAP, FAR["y"] + 4096 * 8192 - 16),
+                                   (OVERLAP, FAR["x"]), (OVERLAP, FAR["W"] - 16), (OVERLAP, FAR["bias"]), (OVERLAP, FAR["res"])])
+def test_linear_refuses_workspaces(lib, rc, ws):
+    """The kernels store into the workspace 16 bytes at a time: a slice of one that starts elsewhere would fault."""
+    nbytes = lib.rl_linear_workspace_bytes(4096, 4096, 4096)
+    assert nbytes > 0
+    assert call_linear(lib, ws=ws, ws_bytes=nbytes, **BIG) == rc
+
+
+@no_gpu
+def test_linear_accepts_an_aligned_workspace(lib):
+    assert passed(call_linear(lib, ws=0x10000000010, ws_bytes=lib.rl_linear_workspace_bytes(4096, 4096, 4096), **BIG))
+
+
 @no_gpu
 def test_linear_accepts(lib):
     assert passed(call_linear(lib))
