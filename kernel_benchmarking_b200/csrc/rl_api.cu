@@ -534,38 +534,50 @@ int launch_decode(const void* x, const __nv_bfloat16* gamma, const void* W, void
 // ---- the cluster-split kernel of the linear layer
 struct SplitPlan {
   int nt, split;  // tokens per tile, CTAs per cluster; nt = 0: the CTA-pair kernel
+  bool deep;      // the long ring, one CTA per SM
 };
-// Cluster-split kernel or CTA pairs, and the former's tile and cluster size: the least of what a short model says, in
-// microseconds.  Its figures are fits to measurements of 36 shapes with every tile and cluster size (tokens 1..4096, K
-// 256..14336): 4.5 us for a launch, its pipeline's start and its exchange, 5.9 where SMs take a second CTA, which starts a
-// microsecond later (1 more for 128-token tiles, 0.05 per part, 0.012 per token that a CTA finishes), and the k-blocks at
-// 160 KB/us an SM with two CTAs on it, 100 with one.  So 64 x 4096 x 4096 runs in 128 CTAs (10.7 us) rather than 256 (12.0), 333 x 1000 x 1144 in 96 (6.8)
-// rather than 192 (8.0), 128 x 4096 x 4096 in 256 (12.7) rather than 128 (14.0).  The pairs: 10 us (8 without an epilogue, 12
-// with everything), and 0.34 per k-block of a round of tiles.  Measured, split against pairs: 128 x 4096 x 4096 12.6 / 20.4
-// us, 512 x 4096 x 4096 20.7 / 23.4, 1024^3 8.0 / 12.6, 1500 x 1536 x 1536 12.7 / 16.0, 4096 x 512 x 256 6.6 / 8.7; the
-// other way round 512 x 4096 x 14336 58 / 53, 1024 x 4096 x 4096 34.7 / 29.9.  Up to 64 tokens it is always the former
-// (against the weight-streaming kernel of the norm: 16 x 4096 x 4096 9.0 / 13.2 us, 64 x 14336 x 4096 23.4 / 32, 64 x
-// 28672 x 4096 41.4 / 45.5).  The plan is arithmetic on the sizes, for the 148 SMs of a B200.
+// Cluster-split kernel or CTA pairs, and the former's tile, cluster size and ring: the least of what a short model says, in
+// microseconds.  Its figures are fits to measurements of 55 shapes with every tile, cluster size and ring (tokens 1..4096, K
+// 256..14336; what it picks is 1.2 % slower than the best of each, 17 % at worst).  3.3 us for launch, start and exchange,
+// 2.2 more where SMs take a second CTA, 0.8 for the long ring; the k-blocks at 86 KB/us an SM, 144 with two CTAs on it, 115
+// with the long ring; 0.024 per token that a CTA finishes; (0.0074 per token of a tile, less 0.3) for every further CTA of a
+// cluster.  Clusters that do not all fit at once would run in two rounds (700 x 1536 x 6144 in 288 CTAs of clusters of 4
+// 27.4 us, in 144 of clusters of 2 19.2), so they are not considered.  The pairs: 8.8 us and 0.33 per k-block of a round of
+// tiles.  Measured, split against pairs: 128 x 4096 x 4096 12.4 / 20 us, 256 x 4096 x 4096 15.1 / 20.6, 512 x 4096 x 4096
+// 21.6 / 23.8, 1024^3 8.3 / 12.6, 4096 x 512 x 256 7.2 / 9.8; the other way round 512 x 4096 x 14336 58 / 52, 1024 x 4096 x
+// 4096 34.7 / 30.9.  Up to 64 tokens it is always the former (against the weight-streaming kernel of the norm: 16 x 4096 x
+// 4096 9.0 / 13.2 us, 64 x 14336 x 4096 23.4 / 32, 64 x 28672 x 4096 41.4 / 45.5).  The plan is arithmetic on the sizes, for
+// the 148 SMs of a B200.
 SplitPlan plan_split(int M, int N, int K) {
   constexpr int SMS = 148, PAIRS = 74;
+  // CTAs that run at once in clusters of 1, 2, 4 and 8, with one and with two on an SM (an SM or two of a GPC are left over)
+  constexpr int ONE[4] = {SMS, SMS, 132, 120}, TWO[4] = {2 * SMS, 2 * SMS, 284, 248};
   const int KB = (K + 63) / 64;
-  SplitPlan best{0, 1};
+  SplitPlan best{0, 1, false};
   double best_us = 1e30;
   const int nt_first = M <= 16 ? 16 : (M <= 32 ? 32 : 64), nt_last = M <= 64 ? nt_first : 128;
   for (int nt = nt_first; nt <= nt_last; nt *= 2) {
     const long long tiles = (long long)((M + nt - 1) / nt) * ((N + 127) / 128);
-    for (int s = 1; s <= 8 && (s == 1 || (tiles * s <= 2 * SMS && KB >= 2 * s)); s *= 2) {
-      const long long ctas = tiles * s, per_sm = (ctas + SMS - 1) / SMS;
-      if (M > 64 && per_sm > 2) break;
-      const double kb_us = (16.0 + nt / 8.0) / (per_sm >= 2 ? 160.0 : 100.0);
-      const double us = (per_sm >= 2 ? 5.9 : 4.5) + (double)per_sm * ((KB + s - 1) / s) * kb_us + 0.05 * s + 0.012 * nt / s +
-                        (nt == 128 ? 1.0 : 0.0);
-      if (us < best_us) { best_us = us; best = SplitPlan{nt, s}; }
+    const double kb_kbytes = 16.0 + nt / 8.0;  // of one k-block
+    for (int l = 0; l < 4; ++l) {
+      const int s = 1 << l;
+      const long long ctas = tiles * s;
+      if (s > 1 && KB < 2 * s) break;
+      const double us = 3.3 + 0.024 * nt / s + (0.0074 * nt - 0.3) * (s - 1), stream = (KB + s - 1) / s * kb_kbytes;
+      if (ctas <= TWO[l] || (M <= 64 && s == 1)) {
+        const long long per_sm = std::max(2LL, (ctas + SMS - 1) / SMS);
+        const double t = us + (ctas <= ONE[l] ? stream / 86.0 : 2.2 + (double)per_sm * stream / 144.0);
+        if (t < best_us) { best_us = t; best = SplitPlan{nt, s, false}; }
+      }
+      if (nt >= 64 && ctas <= ONE[l]) {
+        const double t = us + 0.8 + stream / 115.0;
+        if (t < best_us) { best_us = t; best = SplitPlan{nt, s, true}; }
+      }
     }
   }
   if (M > 64) {
     const long long tiles = (long long)((M + 255) / 256) * ((N + 255) / 256);
-    if (10.0 + 0.34 * KB * rounds_cost(tiles, PAIRS, KB) < best_us) return SplitPlan{0, 1};
+    if (8.8 + 0.33 * KB * rounds_cost(tiles, PAIRS, KB) < best_us) return SplitPlan{0, 1, false};
   }
   return best;
 }
@@ -1227,8 +1239,8 @@ int rl_linear_bf16(const rl_linear_args* args, void* stream) {
     switch (plan.nt) {
       case 16: return launch_split<SplitCfg<16, 6>>(pa, plan.split);
       case 32: return launch_split<SplitCfg<32, 5>>(pa, plan.split);
-      case 64: return launch_split<SplitCfg<64, 4>>(pa, plan.split);
-      default: return launch_split<SplitCfg<128, 3>>(pa, plan.split);
+      case 64: return plan.deep ? launch_split<SplitCfg<64, 8>>(pa, plan.split) : launch_split<SplitCfg<64, 4>>(pa, plan.split);
+      default: return plan.deep ? launch_split<SplitCfg<128, 6>>(pa, plan.split) : launch_split<SplitCfg<128, 3>>(pa, plan.split);
     }
   }
   // The 256 x 512 tiles' epilogue is not hidden behind the next tile's main loop as the 256 x 256 tiles' is.  Measured, it
