@@ -78,6 +78,22 @@ def test_linear(M, N, K, act, bias, residual):
     check_linear(y, x, W, b, act, r)
 
 
+@pytest.mark.parametrize("M,N,K", [
+    (148, 4874, 808), (66, 2110, 1720), (1003, 19, 4464), (40, 14, 5800),    # 64-token tiles, long ring, clusters of 1, 2, 4, 8
+    (387, 2845, 528), (83, 4829, 1104), (82, 2305, 3696),                    # 128-token tiles, long ring, clusters of 1, 2, 4
+    (971, 1929, 72), (222, 2485, 512), (265, 1948, 4528),                    # 128-token tiles, two CTAs on an SM
+    (64, 4097, 112), (64, 4916, 328), (40, 4136, 2176), (40, 10, 1968)])     # 64-token tiles, two CTAs on an SM
+@pytest.mark.parametrize("act,bias,residual", [("gelu", True, True), (None, False, False)])
+def test_linear_of_few_tiles(M, N, K, act, bias, residual):
+    """Every tile, cluster size and ring of the cluster kernel, with ragged last tiles, twice with the same result."""
+    x, W, b, r = linear_inputs(M, N, K, 25, bias, residual)
+    y = kb.linear(x, W, b, activation=act, residual=r)
+    again = kb.linear(x, W, b, activation=act, residual=r)
+    done()
+    check_linear(y, x, W, b, act, r)
+    assert torch.equal(y, again)
+
+
 @pytest.mark.parametrize("M,N,K", [(4096, 1536, 4096),      # 96 tiles: one round, 22 cut in three
                                    (2048, 5120, 2048),      # a last round cut in four
                                    (8192, 7168, 4096),      # 256 x 512 tiles
